@@ -63,7 +63,8 @@ int wush_init(void);
  * variants, wush_w4a4_gemm_tensor_scale_ws) use word 0 of that scratch.  The kernels without caller
  * scratch use library-owned device words, which this call (synchronous: it copies a few bytes from
  * the device) returns in *flag and clears: bits 0-7 the role code left by a streaming (DECODE)
- * kernel, bits 8-15 the role code left by a kernel of wush_w4a4_gemm_static_scratch.
+ * kernel, bits 8-15 the role code left by a kernel of wush_w4a4_gemm_static_scratch,
+ * bits 16-23 the role code left by a kernel of the 8-bit products (wush_w8a8_*).
  * 0 means no such kernel gave up since the last call. */
 int wush_device_flag(int* flag);
 
@@ -221,6 +222,78 @@ size_t wush_w4a4_gemm_tensor_scale_workspace_bytes(int64_t M, int64_t N, int64_t
 int wush_w4a4_gemm_tensor_scale_ws(const uint8_t* xq, const uint8_t* wq, int64_t M, int64_t N,
                                    int64_t K, float alpha, const float* alpha_dev, void* y,
                                    void* workspace, size_t workspace_bytes, void* stream);
+
+/* --- 8-bit layers (no counterpart in the reference) ---------------------------------------------
+ * For layers whose accuracy does not bear 4 bits: the same layer with int8 codes, one fp32 scale per
+ * activation row and one per weight row (output channel), and the mixture-of-experts feed-forward
+ * block built on its grouped form.
+ *   codes   int8, row-major, 16-byte aligned, K % 16 == 0, K <= WUSH_W8A8_MAX_K
+ *   scales  fp32, one per row
+ * Element types of activations and results: */
+typedef enum { WUSH_BF16 = 0, WUSH_F16 = 1, WUSH_F32 = 2 } wush_dtype;
+#define WUSH_W8A8_MAX_K 131072   /* the int32 sum of K products of codes up to 127 in magnitude does not overflow */
+#define WUSH_EXPERT_MAX 1024     /* experts of one block */
+#define WUSH_EXPERT_MAX_K 64     /* experts of one token */
+
+/* s = amax(|row|) / 127, q = rint(127 * x / amax(|row|)), ties to even; exactly so for bf16 and fp16
+ * rows (fp32 rows: x * fl(127 / amax), a last-place difference at ties).  An all-zero row has s = 0 and
+ * codes 0; a row that holds an infinity or a NaN has that as its s and codes 0.
+ * x: rows*K of `dtype`, 16-byte aligned;  q: rows*K, 16-byte aligned;  s: rows. */
+int wush_quant_int8(const void* x, int dtype, int64_t rows, int64_t K, int8_t* q, float* s, void* stream);
+
+/* y[m][n] = xs[m] * ws[n] * sum_k xq[m][k] * wq[n][k] (+ bias[n]), exact int32 sums, scales in fp32, one
+ * rounding to `out_dtype` (WUSH_F16 or WUSH_BF16).  bias: N fp32 or NULL.  No scratch. */
+int wush_w8a8_gemm(const int8_t* xq, const float* xs, const int8_t* wq, const float* ws, const float* bias,
+                   int64_t M, int64_t N, int64_t K, void* y, int out_dtype, void* stream);
+
+/* The two in one call: quantise x (M, K) of `dtype` (WUSH_F16 or WUSH_BF16) into the workspace, then the
+ * product, whose kernel fetches its first weights while the quantiser runs.  y has the type of x. */
+size_t wush_w8a8_linear_workspace_bytes(int64_t M, int64_t K);
+int wush_w8a8_linear(const void* x, int dtype, const int8_t* wq, const float* ws, const float* bias, int64_t M,
+                     int64_t N, int64_t K, void* y, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Tokens ordered by expert.  An entry is a pair (token t, choice j < k); R = tokens * k.
+ *   ids      (tokens, k) int32 or int64 (`id_bytes` 4 or 8): an id outside [0, experts) names no expert
+ *   pos      (tokens, k) int32: row of the entry among the entries sorted by expert, stable in t * k + j;
+ *            -1 where there is no expert
+ *   offsets  (experts + 1) int32: first row of each expert; offsets[experts] = number of entries
+ * gather: rows[pos] = x[t]; the R - offsets[experts] rows behind the last entry become zero.
+ * combine: y[t] = sum over j of weights[t][j] * rows[pos[t][j]], fp32 sums in ascending j, entries with
+ *   pos -1 neither read nor weighted; weights NULL = ones, which is the gradient of gather.
+ * combine_grad: d_rows[pos] = weights * dy[t] (rows behind the last entry zero), d_weights[t][j] =
+ *   <dy[t], rows[pos]> in fp32 (0 where there is no expert).
+ * No result depends on an order of execution.  H: any length; rows that are a multiple of 16 bytes at
+ * 16-byte aligned pointers move in 16-byte pieces.  A position outside [0, R) counts as -1. */
+int wush_expert_sort(const void* ids, int id_bytes, int64_t tokens, int64_t k, int64_t experts, int32_t* pos,
+                     int32_t* offsets, void* stream);
+int wush_expert_gather(const void* x, int dtype, int64_t tokens, int64_t H, const int32_t* pos, int64_t k,
+                       const int32_t* offsets, int64_t experts, void* rows, void* stream);
+int wush_expert_gather_quant_int8(const void* x, int dtype, int64_t tokens, int64_t K, const int32_t* pos, int64_t k,
+                                  const int32_t* offsets, int64_t experts, int8_t* q, float* s, void* stream);
+int wush_expert_combine(const void* rows, int dtype, int64_t tokens, int64_t H, const int32_t* pos, int64_t k,
+                        const float* weights, void* y, void* stream);
+int wush_expert_combine_grad(const void* dy, const void* rows, int dtype, int64_t tokens, int64_t H, const int32_t* pos,
+                             int64_t k, const int32_t* offsets, int64_t experts, const float* weights, void* d_rows,
+                             float* d_weights, void* stream);
+
+/* Products grouped by expert: rows [offsets[e], offsets[e + 1]) of xq with the weights of expert e
+ * (wq (experts, N, K), ws (experts, N)); rows from offsets[experts] on become zero.
+ *   gemm   as wush_w8a8_gemm without bias
+ *   gated  wq (experts, 2 * I, K), the I gate channels first: h[m][i] = silu(g) * u in fp32 (rows, I), with g and
+ *          u the products of channels i and I + i.  The result keeps fp32: it is what the next quantiser reads */
+int wush_w8a8_grouped_gemm(const int8_t* xq, const float* xs, const int8_t* wq, const float* ws, const int32_t* offsets,
+                           int64_t rows, int64_t experts, int64_t N, int64_t K, void* y, int out_dtype, void* stream);
+int wush_w8a8_grouped_gated(const int8_t* xq, const float* xs, const int8_t* wq, const float* ws, const int32_t* offsets,
+                            int64_t rows, int64_t experts, int64_t I, int64_t K, float* h, void* stream);
+
+/* The whole block: sort, gather + quantise, gated product, quantise, product, weighted sum.
+ * x, y: (tokens, H) of `dtype` (WUSH_F16 or WUSH_BF16); weights (tokens, k) fp32; w13q (experts, 2 * I, H),
+ * w13s (experts, 2 * I), w2q (experts, H, I), w2s (experts, H).  The experts' outputs are rounded to `dtype`
+ * before the weighted sum, which is fp32. */
+size_t wush_w8a8_expert_ffn_workspace_bytes(int64_t tokens, int64_t H, int64_t I, int64_t experts, int64_t k);
+int wush_w8a8_expert_ffn(const void* x, int dtype, const void* ids, int id_bytes, const float* weights, const int8_t* w13q,
+                         const float* w13s, const int8_t* w2q, const float* w2s, int64_t tokens, int64_t H, int64_t I,
+                         int64_t experts, int64_t k, void* y, void* workspace, size_t workspace_bytes, void* stream);
 
 /* --- multi-GPU: one-shot all-reduce of small fp16 partial products over NVLink peer memory ------
  * No counterpart in the reference (single GPU).  The row-parallel down projection of a

@@ -6,7 +6,8 @@ Layout
     _C                     compiled torch-facing operator module (same surface as the reference's ``my_int4._C``)
     rtn_int4.py            torch reference semantics of the quantiser (mirrors ``my_int4/rtn_int4.py``)
     wush_transform.py      offline transform solve / weight transform (mirrors ``my_int4/wush_transform.py``)
-    linear.py              M-dispatching W4A4 linear layer and its N-sharded variant
+    linear.py              M-dispatching W4A4 linear layer and its N-sharded variant; the 8-bit layer
+    experts.py             tokens ordered by expert (with gradients) and the 8-bit mixture-of-experts block
 
 The compiled pieces are required: importing ``_C`` (or ``my_int4``) without them raises
 ImportError -- there is no CPU fallback.  ``python -m wush_int4_kernel_b200.build`` builds them.

@@ -16,6 +16,8 @@ WUSH_OK = 0
 WUSH_ERR_INVALID_ARGUMENT, WUSH_ERR_CUDA, WUSH_ERR_UNSUPPORTED, WUSH_ERR_WORKSPACE, WUSH_ERR_DEVICE_FLAG = 1, 2, 3, 4, 5
 TQ_EXACT, TQ_FAST = 0, 1
 GEMM_AUTO, GEMM_GEMV, GEMM_DECODE, GEMM_TILE, GEMM_TILE_F16, GEMM_DECODE_TC, GEMM_GEMV_MMA = 0, 1, 2, 3, 4, 5, 6
+BF16, F16, F32 = 0, 1, 2
+W8A8_MAX_K, EXPERT_MAX, EXPERT_MAX_K = 131072, 1024, 64
 
 _vp, _i64, _int, _f32, _sz = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_float, ctypes.c_size_t
 
@@ -38,6 +40,20 @@ SIGNATURES = {
     "wush_group_partials": (_int, [_vp, _vp, _i64, _i64, _i64, _vp, _vp]),
     "wush_quant_int4_tensor_scale": (_int, [_vp, _i64, _f32, _vp, _vp, _vp]),
     "wush_w4a4_gemm_tensor_scale": (_int, [_vp, _vp, _i64, _i64, _i64, _f32, _vp, _vp, _vp]),
+    "wush_quant_int8": (_int, [_vp, _int, _i64, _i64, _vp, _vp, _vp]),
+    "wush_w8a8_gemm": (_int, [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp, _int, _vp]),
+    "wush_w8a8_linear_workspace_bytes": (_sz, [_i64, _i64]),
+    "wush_w8a8_linear": (_int, [_vp, _int, _vp, _vp, _vp, _i64, _i64, _i64, _vp, _vp, _sz, _vp]),
+    "wush_expert_sort": (_int, [_vp, _int, _i64, _i64, _i64, _vp, _vp, _vp]),
+    "wush_expert_gather": (_int, [_vp, _int, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _vp]),
+    "wush_expert_gather_quant_int8": (_int, [_vp, _int, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _vp]),
+    "wush_expert_combine": (_int, [_vp, _int, _i64, _i64, _vp, _i64, _vp, _vp, _vp]),
+    "wush_expert_combine_grad": (_int, [_vp, _vp, _int, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp]),
+    "wush_w8a8_grouped_gemm": (_int, [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _int, _vp]),
+    "wush_w8a8_grouped_gated": (_int, [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _vp]),
+    "wush_w8a8_expert_ffn_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64, _i64]),
+    "wush_w8a8_expert_ffn": (_int, [_vp, _int, _vp, _int, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _vp, _vp,
+                                    _sz, _vp]),
     "wush_comm_create": (_int, [_int, _int, _sz, ctypes.POINTER(ctypes.c_void_p)]),
     "wush_comm_export": (_int, [_vp, _vp]),
     "wush_comm_connect": (_int, [_vp, _int, _vp]),

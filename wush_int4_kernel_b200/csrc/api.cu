@@ -41,6 +41,8 @@ int tc_set_attributes();
 int stream_set_attributes();
 int f16_set_attributes();
 int decode_tc_set_attributes();
+int expert_order_set_attributes();
+int w8a8_set_attributes();
 
 static int init_device(int dev)
 {
@@ -58,6 +60,8 @@ static int init_device(int dev)
     if (int s = stream_set_attributes()) return s;
     if (int s = f16_set_attributes()) return s;
     if (int s = decode_tc_set_attributes()) return s;
+    if (int s = expert_order_set_attributes()) return s;
+    if (int s = w8a8_set_attributes()) return s;
     return WUSH_OK;
 }
 

@@ -271,6 +271,304 @@ torch::Tensor w4a4_gemm_cutlass_dev(torch::Tensor xq, torch::Tensor wq, torch::T
     return gemm_ts(xq, wq, 0.f, alpha.data_ptr<float>(), "w4a4_gemm_cutlass_dev");
 }
 
+// ---- 8-bit layers ---------------------------------------------------------------------
+int dtype_code(const torch::Tensor& t, const char* op, const char* name, bool with_f32)
+{
+    const auto d = t.scalar_type();
+    if (d == torch::kBFloat16) return WUSH_BF16;
+    if (d == torch::kHalf) return WUSH_F16;
+    TORCH_CHECK(with_f32 && d == torch::kFloat32, op, ": ", name, with_f32 ? " must be bf16, fp16 or fp32" : " must be bf16 or fp16");
+    return WUSH_F32;
+}
+
+// A contiguous CUDA tensor on the device of `like`.
+void check_on(const torch::Tensor& t, const torch::Tensor& like, const char* op, const char* name)
+{
+    TORCH_CHECK(t.is_cuda() && t.is_contiguous(), op, ": ", name, " must be a contiguous CUDA tensor");
+    TORCH_CHECK(t.device() == like.device(), op, ": tensors must be on the same device");
+}
+
+void check_type(const torch::Tensor& t, torch::ScalarType d, const char* op, const char* name)
+{
+    TORCH_CHECK(t.scalar_type() == d, op, ": ", name, " must be ", d);
+}
+
+int64_t rows_of(const torch::Tensor& t) { return t.size(-1) ? t.numel() / t.size(-1) : 0; }
+
+std::vector<int64_t> without_last(const torch::Tensor& t)
+{
+    std::vector<int64_t> s = t.sizes().vec();
+    s.pop_back();
+    return s;
+}
+
+std::vector<torch::Tensor> quant_int8(torch::Tensor x)
+{
+    check_on(x, x, "quant_int8", "x");
+    const int dt = dtype_code(x, "quant_int8", "x", true);
+    TORCH_CHECK(x.dim() >= 1 && x.size(-1) > 0 && x.size(-1) % 16 == 0, "quant_int8: last dim must be a multiple of 16");
+    const at::cuda::OptionalCUDAGuard guard(x.device());
+    auto q = torch::empty(x.sizes(), x.options().dtype(torch::kInt8));
+    auto s = torch::empty(without_last(x), x.options().dtype(torch::kFloat32));
+    check_status(wush_quant_int8(x.data_ptr(), dt, rows_of(x), x.size(-1), q.data_ptr<int8_t>(), s.data_ptr<float>(), stream_of(x)),
+                 "quant_int8");
+    return {q, s};
+}
+
+// Codes (..., K) with their scales (...).
+void check_codes(const torch::Tensor& q, const torch::Tensor& s, const torch::Tensor& like, const char* op, const char* qn, const char* sn)
+{
+    check_on(q, like, op, qn);
+    check_on(s, like, op, sn);
+    check_type(q, torch::kInt8, op, qn);
+    check_type(s, torch::kFloat32, op, sn);
+    TORCH_CHECK(q.dim() >= 1 && q.sizes().slice(0, q.dim() - 1) == s.sizes(), op, ": ", sn, " must have the shape of ", qn,
+                " without its last dimension");
+}
+
+const float* check_bias(const c10::optional<torch::Tensor>& bias, const torch::Tensor& like, int64_t N, const char* op)
+{
+    if (!bias.has_value()) return nullptr;
+    check_on(*bias, like, op, "bias");
+    check_type(*bias, torch::kFloat32, op, "bias");
+    TORCH_CHECK(bias->dim() == 1 && bias->size(0) == N, op, ": bias must be (N)");
+    return bias->data_ptr<float>();
+}
+
+int out_code(torch::ScalarType d, const char* op)
+{
+    TORCH_CHECK(d == torch::kHalf || d == torch::kBFloat16, op, ": out_dtype must be torch.float16 or torch.bfloat16");
+    return d == torch::kHalf ? WUSH_F16 : WUSH_BF16;
+}
+
+torch::Tensor w8a8_gemm(torch::Tensor xq, torch::Tensor xs, torch::Tensor wq, torch::Tensor ws, c10::optional<torch::Tensor> bias,
+                        torch::ScalarType out_dtype)
+{
+    const char* op = "w8a8_gemm";
+    check_codes(xq, xs, xq, op, "xq", "xs");
+    check_codes(wq, ws, xq, op, "wq", "ws");
+    TORCH_CHECK(wq.dim() == 2, op, ": wq must be (N, K)");
+    const int64_t N = wq.size(0), K = wq.size(1);
+    TORCH_CHECK(K > 0 && xq.size(-1) == K, op, ": K mismatch between xq and wq");
+    const int code = out_code(out_dtype, op);
+    const at::cuda::OptionalCUDAGuard guard(xq.device());
+    auto y = torch::empty(with_last(xq, N), xq.options().dtype(out_dtype));
+    check_status(wush_w8a8_gemm(xq.data_ptr<int8_t>(), xs.data_ptr<float>(), wq.data_ptr<int8_t>(), ws.data_ptr<float>(),
+                                check_bias(bias, xq, N, op), xq.numel() / K, N, K, y.data_ptr(), code, stream_of(xq)),
+                 op);
+    return y;
+}
+
+torch::Tensor w8a8_linear(torch::Tensor x, torch::Tensor wq, torch::Tensor ws, c10::optional<torch::Tensor> bias)
+{
+    const char* op = "w8a8_linear";
+    check_on(x, x, op, "x");
+    const int dt = dtype_code(x, op, "x", false);
+    check_codes(wq, ws, x, op, "wq", "ws");
+    TORCH_CHECK(wq.dim() == 2 && x.dim() >= 1, op, ": wq must be (N, K)");
+    const int64_t N = wq.size(0), K = wq.size(1);
+    TORCH_CHECK(K > 0 && x.size(-1) == K, op, ": K mismatch between x and wq");
+    const int64_t M = x.numel() / K;
+    const at::cuda::OptionalCUDAGuard guard(x.device());
+    auto y = torch::empty(with_last(x, N), x.options());
+    const size_t nbytes = wush_w8a8_linear_workspace_bytes(M, K);
+    auto work = torch::empty({(int64_t)nbytes}, x.options().dtype(torch::kUInt8));
+    check_status(wush_w8a8_linear(x.data_ptr(), dt, wq.data_ptr<int8_t>(), ws.data_ptr<float>(), check_bias(bias, x, N, op), M, N, K,
+                                  y.data_ptr(), work.data_ptr(), nbytes, stream_of(x)),
+                 op);
+    return y;
+}
+
+// ---- tokens ordered by expert -----------------------------------------------------------
+int id_bytes_of(const torch::Tensor& ids, const char* op)
+{
+    TORCH_CHECK(ids.scalar_type() == torch::kInt32 || ids.scalar_type() == torch::kInt64, op, ": ids must be int32 or int64");
+    return ids.scalar_type() == torch::kInt64 ? 8 : 4;
+}
+
+struct Route {
+    int64_t tokens, k, experts;
+};
+
+Route check_route(const torch::Tensor& pos, const torch::Tensor& offsets, const torch::Tensor& like, const char* op)
+{
+    check_on(pos, like, op, "pos");
+    check_on(offsets, like, op, "offsets");
+    check_type(pos, torch::kInt32, op, "pos");
+    check_type(offsets, torch::kInt32, op, "offsets");
+    TORCH_CHECK(pos.dim() == 2 && pos.size(1) >= 1, op, ": pos must be (tokens, k)");
+    TORCH_CHECK(offsets.dim() == 1 && offsets.size(0) >= 2, op, ": offsets must be (experts + 1)");
+    return {pos.size(0), pos.size(1), offsets.size(0) - 1};
+}
+
+std::vector<torch::Tensor> expert_sort(torch::Tensor ids, int64_t n_experts)
+{
+    const char* op = "expert_sort";
+    check_on(ids, ids, op, "ids");
+    const int bytes = id_bytes_of(ids, op);
+    TORCH_CHECK(ids.dim() == 2, op, ": ids must be (tokens, k)");
+    TORCH_CHECK(n_experts >= 1 && n_experts <= WUSH_EXPERT_MAX, op, ": takes 1..", WUSH_EXPERT_MAX, " experts (got ", n_experts, ")");
+    const at::cuda::OptionalCUDAGuard guard(ids.device());
+    auto pos = torch::empty(ids.sizes(), ids.options().dtype(torch::kInt32));
+    auto offsets = torch::empty({n_experts + 1}, ids.options().dtype(torch::kInt32));
+    check_status(wush_expert_sort(ids.data_ptr(), bytes, ids.size(0), ids.size(1), n_experts, pos.data_ptr<int32_t>(),
+                                  offsets.data_ptr<int32_t>(), stream_of(ids)),
+                 op);
+    return {pos, offsets};
+}
+
+torch::Tensor expert_gather(torch::Tensor x, torch::Tensor pos, torch::Tensor offsets)
+{
+    const char* op = "expert_gather";
+    check_on(x, x, op, "x");
+    const int dt = dtype_code(x, op, "x", true);
+    const Route r = check_route(pos, offsets, x, op);
+    TORCH_CHECK(x.dim() == 2 && x.size(0) == r.tokens && x.size(1) >= 1, op, ": x must be (tokens, H) with the tokens of pos");
+    const at::cuda::OptionalCUDAGuard guard(x.device());
+    auto rows = torch::empty({r.tokens * r.k, x.size(1)}, x.options());
+    check_status(wush_expert_gather(x.data_ptr(), dt, r.tokens, x.size(1), pos.data_ptr<int32_t>(), r.k, offsets.data_ptr<int32_t>(),
+                                    r.experts, rows.data_ptr(), stream_of(x)),
+                 op);
+    return rows;
+}
+
+std::vector<torch::Tensor> expert_gather_quant_int8(torch::Tensor x, torch::Tensor pos, torch::Tensor offsets)
+{
+    const char* op = "expert_gather_quant_int8";
+    check_on(x, x, op, "x");
+    const int dt = dtype_code(x, op, "x", true);
+    const Route r = check_route(pos, offsets, x, op);
+    TORCH_CHECK(x.dim() == 2 && x.size(0) == r.tokens && x.size(1) > 0 && x.size(1) % 16 == 0, op,
+                ": x must be (tokens, K) with the tokens of pos, K a multiple of 16");
+    const at::cuda::OptionalCUDAGuard guard(x.device());
+    auto q = torch::empty({r.tokens * r.k, x.size(1)}, x.options().dtype(torch::kInt8));
+    auto s = torch::empty({r.tokens * r.k}, x.options().dtype(torch::kFloat32));
+    check_status(wush_expert_gather_quant_int8(x.data_ptr(), dt, r.tokens, x.size(1), pos.data_ptr<int32_t>(), r.k,
+                                               offsets.data_ptr<int32_t>(), r.experts, q.data_ptr<int8_t>(), s.data_ptr<float>(),
+                                               stream_of(x)),
+                 op);
+    return {q, s};
+}
+
+void check_weights(const torch::Tensor& w, const torch::Tensor& pos, const torch::Tensor& like, const char* op)
+{
+    check_on(w, like, op, "weights");
+    check_type(w, torch::kFloat32, op, "weights");
+    TORCH_CHECK(w.sizes() == pos.sizes(), op, ": weights must be (tokens, k)");
+}
+
+torch::Tensor expert_combine(torch::Tensor rows, torch::Tensor pos, c10::optional<torch::Tensor> weights)
+{
+    const char* op = "expert_combine";
+    check_on(rows, rows, op, "rows");
+    const int dt = dtype_code(rows, op, "rows", true);
+    check_on(pos, rows, op, "pos");
+    check_type(pos, torch::kInt32, op, "pos");
+    TORCH_CHECK(pos.dim() == 2 && pos.size(1) >= 1, op, ": pos must be (tokens, k)");
+    TORCH_CHECK(rows.dim() == 2 && rows.size(0) == pos.numel() && rows.size(1) >= 1, op, ": rows must be (tokens * k, H)");
+    if (weights.has_value()) check_weights(*weights, pos, rows, op);
+    const at::cuda::OptionalCUDAGuard guard(rows.device());
+    auto y = torch::empty({pos.size(0), rows.size(1)}, rows.options());
+    check_status(wush_expert_combine(rows.data_ptr(), dt, pos.size(0), rows.size(1), pos.data_ptr<int32_t>(), pos.size(1),
+                                     weights.has_value() ? weights->data_ptr<float>() : nullptr, y.data_ptr(), stream_of(rows)),
+                 op);
+    return y;
+}
+
+std::vector<torch::Tensor> expert_combine_grad(torch::Tensor dy, torch::Tensor rows, torch::Tensor pos, torch::Tensor offsets,
+                                               torch::Tensor weights)
+{
+    const char* op = "expert_combine_grad";
+    check_on(rows, rows, op, "rows");
+    const int dt = dtype_code(rows, op, "rows", true);
+    check_on(dy, rows, op, "dy");
+    check_type(dy, rows.scalar_type(), op, "dy");
+    const Route r = check_route(pos, offsets, rows, op);
+    TORCH_CHECK(rows.dim() == 2 && rows.size(0) == r.tokens * r.k && rows.size(1) >= 1, op, ": rows must be (tokens * k, H)");
+    TORCH_CHECK(dy.dim() == 2 && dy.size(0) == r.tokens && dy.size(1) == rows.size(1), op, ": dy must be (tokens, H)");
+    check_weights(weights, pos, rows, op);
+    const at::cuda::OptionalCUDAGuard guard(rows.device());
+    auto d_rows = torch::empty_like(rows);
+    auto d_weights = torch::empty_like(weights);
+    check_status(wush_expert_combine_grad(dy.data_ptr(), rows.data_ptr(), dt, r.tokens, rows.size(1), pos.data_ptr<int32_t>(), r.k,
+                                          offsets.data_ptr<int32_t>(), r.experts, weights.data_ptr<float>(), d_rows.data_ptr(),
+                                          d_weights.data_ptr<float>(), stream_of(rows)),
+                 op);
+    return {d_rows, d_weights};
+}
+
+struct Grouped {
+    int64_t rows, experts, N, K;
+};
+
+Grouped check_grouped(const torch::Tensor& xq, const torch::Tensor& xs, const torch::Tensor& wq, const torch::Tensor& ws,
+                      const torch::Tensor& offsets, const char* op)
+{
+    check_codes(xq, xs, xq, op, "xq", "xs");
+    check_codes(wq, ws, xq, op, "wq", "ws");
+    check_on(offsets, xq, op, "offsets");
+    check_type(offsets, torch::kInt32, op, "offsets");
+    TORCH_CHECK(xq.dim() == 2 && wq.dim() == 3 && xq.size(1) > 0 && xq.size(1) == wq.size(2), op, ": xq must be (rows, K), wq (experts, N, K)");
+    TORCH_CHECK(offsets.dim() == 1 && offsets.size(0) == wq.size(0) + 1, op, ": offsets must be (experts + 1)");
+    return {xq.size(0), wq.size(0), wq.size(1), xq.size(1)};
+}
+
+torch::Tensor w8a8_grouped_gemm(torch::Tensor xq, torch::Tensor xs, torch::Tensor wq, torch::Tensor ws, torch::Tensor offsets,
+                                torch::ScalarType out_dtype)
+{
+    const char* op = "w8a8_grouped_gemm";
+    const Grouped g = check_grouped(xq, xs, wq, ws, offsets, op);
+    const int code = out_code(out_dtype, op);
+    const at::cuda::OptionalCUDAGuard guard(xq.device());
+    auto y = torch::empty({g.rows, g.N}, xq.options().dtype(out_dtype));
+    check_status(wush_w8a8_grouped_gemm(xq.data_ptr<int8_t>(), xs.data_ptr<float>(), wq.data_ptr<int8_t>(), ws.data_ptr<float>(),
+                                        offsets.data_ptr<int32_t>(), g.rows, g.experts, g.N, g.K, y.data_ptr(), code, stream_of(xq)),
+                 op);
+    return y;
+}
+
+torch::Tensor w8a8_grouped_gated(torch::Tensor xq, torch::Tensor xs, torch::Tensor wq, torch::Tensor ws, torch::Tensor offsets)
+{
+    const char* op = "w8a8_grouped_gated";
+    const Grouped g = check_grouped(xq, xs, wq, ws, offsets, op);
+    TORCH_CHECK(g.N % 2 == 0, op, ": wq must be (experts, 2 * I, K), the gate channels first");
+    const at::cuda::OptionalCUDAGuard guard(xq.device());
+    auto h = torch::empty({g.rows, g.N / 2}, xq.options().dtype(torch::kFloat32));
+    check_status(wush_w8a8_grouped_gated(xq.data_ptr<int8_t>(), xs.data_ptr<float>(), wq.data_ptr<int8_t>(), ws.data_ptr<float>(),
+                                         offsets.data_ptr<int32_t>(), g.rows, g.experts, g.N / 2, g.K, h.data_ptr<float>(),
+                                         stream_of(xq)),
+                 op);
+    return h;
+}
+
+torch::Tensor w8a8_expert_ffn(torch::Tensor x, torch::Tensor ids, torch::Tensor weights, torch::Tensor w13q, torch::Tensor w13s,
+                              torch::Tensor w2q, torch::Tensor w2s)
+{
+    const char* op = "w8a8_expert_ffn";
+    check_on(x, x, op, "x");
+    const int dt = dtype_code(x, op, "x", false);
+    check_on(ids, x, op, "ids");
+    const int bytes = id_bytes_of(ids, op);
+    TORCH_CHECK(x.dim() == 2 && ids.dim() == 2 && ids.size(0) == x.size(0) && ids.size(1) >= 1, op,
+                ": x must be (tokens, H) and ids (tokens, k)");
+    check_weights(weights, ids, x, op);
+    check_codes(w13q, w13s, x, op, "w13q", "w13s");
+    check_codes(w2q, w2s, x, op, "w2q", "w2s");
+    const int64_t T = x.size(0), H = x.size(1), k = ids.size(1);
+    TORCH_CHECK(w13q.dim() == 3 && w13q.size(2) == H && w13q.size(1) % 2 == 0, op, ": w13q must be (experts, 2 * I, H)");
+    const int64_t E = w13q.size(0), I = w13q.size(1) / 2;
+    TORCH_CHECK(w2q.dim() == 3 && w2q.size(0) == E && w2q.size(1) == H && w2q.size(2) == I, op, ": w2q must be (experts, H, I)");
+    const at::cuda::OptionalCUDAGuard guard(x.device());
+    auto y = torch::empty_like(x);
+    const size_t nbytes = wush_w8a8_expert_ffn_workspace_bytes(T, H, I, E, k);
+    auto work = torch::empty({(int64_t)nbytes}, x.options().dtype(torch::kUInt8));
+    check_status(wush_w8a8_expert_ffn(x.data_ptr(), dt, ids.data_ptr(), bytes, weights.data_ptr<float>(), w13q.data_ptr<int8_t>(),
+                                      w13s.data_ptr<float>(), w2q.data_ptr<int8_t>(), w2s.data_ptr<float>(), T, H, I, E, k, y.data_ptr(),
+                                      work.data_ptr(), nbytes, stream_of(x)),
+                 op);
+    return y;
+}
+
 void init() { check_status(wush_init(), "init"); }
 
 }  // namespace
@@ -312,6 +610,28 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
           py::arg("xs"), py::arg("wq"), py::arg("ws"));
     m.def("fused_transform_quant_int4_wmma", &fused_transform_quant_int4_wmma,
           "Fused WUSH transform + INT4 quantise (tensor-core transform)", py::arg("x"), py::arg("t"));
+    // 8-bit layers and experts
+    m.def("quant_int8", &quant_int8, "rows to int8 codes with one fp32 scale per row (bf16 / fp16 / fp32 input)", py::arg("x"));
+    m.def("w8a8_gemm", &w8a8_gemm, "W8A8 product with scales per token and channel, keeps leading dims", py::arg("xq"), py::arg("xs"),
+          py::arg("wq"), py::arg("ws"), py::arg("bias") = py::none(), py::arg("out_dtype") = torch::kHalf);
+    m.def("w8a8_linear", &w8a8_linear, "quant_int8 of x, then w8a8_gemm; the result has the type of x", py::arg("x"), py::arg("wq"),
+          py::arg("ws"), py::arg("bias") = py::none());
+    m.def("expert_sort", &expert_sort, "(tokens, k) expert ids -> row of each entry sorted by expert, first row of each expert",
+          py::arg("ids"), py::arg("n_experts"));
+    m.def("expert_gather", &expert_gather, "rows[pos[t, j]] = x[t]; rows behind the last entry are zero", py::arg("x"), py::arg("pos"),
+          py::arg("offsets"));
+    m.def("expert_gather_quant_int8", &expert_gather_quant_int8, "quant_int8 of x, then expert_gather of codes and scales", py::arg("x"),
+          py::arg("pos"), py::arg("offsets"));
+    m.def("expert_combine", &expert_combine, "y[t] = sum_j weights[t, j] * rows[pos[t, j]] (weights None: ones)", py::arg("rows"),
+          py::arg("pos"), py::arg("weights") = py::none());
+    m.def("expert_combine_grad", &expert_combine_grad, "gradients of expert_combine: (d_rows, d_weights)", py::arg("dy"),
+          py::arg("rows"), py::arg("pos"), py::arg("offsets"), py::arg("weights"));
+    m.def("w8a8_grouped_gemm", &w8a8_grouped_gemm, "w8a8_gemm of each expert's rows with its weights", py::arg("xq"), py::arg("xs"),
+          py::arg("wq"), py::arg("ws"), py::arg("offsets"), py::arg("out_dtype") = torch::kHalf);
+    m.def("w8a8_grouped_gated", &w8a8_grouped_gated, "silu(gate) * up of each expert's rows in fp32, gate channels first", py::arg("xq"),
+          py::arg("xs"), py::arg("wq"), py::arg("ws"), py::arg("offsets"));
+    m.def("w8a8_expert_ffn", &w8a8_expert_ffn, "mixture-of-experts feed-forward block on 8-bit weights", py::arg("x"), py::arg("ids"),
+          py::arg("weights"), py::arg("w13q"), py::arg("w13s"), py::arg("w2q"), py::arg("w2s"));
     // additions of this build
     m.def("w4a4_group_partials", &w4a4_group_partials, "exact int32 partial sums per group (test op)", py::arg("xq"),
           py::arg("wq"));

@@ -1,0 +1,474 @@
+// Tokens ordered by expert and back: the moves around the experts' products of a mixture-of-experts block.
+//
+//   sort      entries (t, j) with expert ids[t, j], by expert and stable in t * k + j:
+//             pos[t, j] = row of the entry (-1 for an id outside [0, E)), offsets[e] = first row of expert e
+//   gather    rows[pos[t, j]] = x[t];  the rows behind the last entry become zero
+//   combine   y[t] = sum_j w[t, j] * rows[pos[t, j]], fp32 sums in ascending j; entries with pos -1 are not read.
+//             Without weights it is the gradient of gather.
+//   grad      of combine: d_rows[pos[t, j]] = w[t, j] * dy[t],  d_w[t, j] = <dy[t], rows[pos[t, j]]> in fp32
+//
+// The moves are bound by memory and written from the token's side: a token's row is read once for all its k entries, and
+// no float is added by an atomic, so that results do not depend on any order of execution.
+#include "common.cuh"
+#include "int8_host.cuh"
+
+namespace wush {
+namespace {
+
+// ---- sort ------------------------------------------------------------------------------------------------------------------
+// A counting sort in one launch of one CTA, or of a cluster of eight that share their counts through distributed shared
+// memory.  Warp w of the cluster owns a contiguous run of the entries, so ranks that ascend inside a run, over the runs
+// of a CTA and over the CTAs are the stable order.  cnt[w][e]: entries of expert e in the run of warp w; then, in place,
+// the row of the warp's next entry of that expert.
+constexpr int SORT_THREADS = 1024, SORT_WARPS = 32, SORT_CLUSTER = 8;
+
+__device__ __forceinline__ uint32_t cluster_rank() { uint32_t r; asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
+__device__ __forceinline__ void cluster_barrier()
+{
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ int32_t ld_cluster_s32(const void* p, uint32_t rank)
+{
+    uint32_t a;
+    int32_t v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
+    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+    return v;
+}
+
+template <typename Id>
+__device__ __forceinline__ int expert_of(const Id* ids, int64_t i, int64_t end, int E)
+{
+    if (i >= end) return -1;
+    const Id v = ids[i];
+    return v >= 0 && v < (Id)E ? (int)v : -1;
+}
+
+template <typename Id, int CTAS>
+__global__ void __launch_bounds__(SORT_THREADS) expert_sort_kernel(const Id* __restrict__ ids, int64_t n, int E,
+                                                                   int32_t* __restrict__ pos, int32_t* __restrict__ offsets)
+{
+    extern __shared__ int32_t sort_smem[];
+    int32_t* cnt = sort_smem;                       // [SORT_WARPS][E]
+    int32_t* total = cnt + SORT_WARPS * E;          // [E]: entries of this CTA; read by the cluster
+    __shared__ int32_t warp_sum[SORT_WARPS];
+    pdl_wait();
+    pdl_launch_dependents();
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const uint32_t rank = CTAS > 1 ? cluster_rank() : 0;
+    // run of this warp: whole rounds of 32 entries, the same number for every warp
+    const int64_t rounds = ((n + 31) / 32 + CTAS * SORT_WARPS - 1) / (CTAS * SORT_WARPS);
+    const int64_t first = ((int64_t)rank * SORT_WARPS + warp) * rounds * 32;
+    const int64_t end = first + rounds * 32 < n ? first + rounds * 32 : n;
+
+    for (int i = tid; i < SORT_WARPS * E; i += SORT_THREADS) cnt[i] = 0;
+    __syncthreads();
+    int32_t* mine = cnt + warp * E;
+    for (int64_t i = first; i < end; i += 32) {
+        const int e = expert_of(ids, i + lane, end, E);
+        const uint32_t same = __match_any_sync(0xffffffffu, e);
+        if (e >= 0 && (same & ((1u << lane) - 1)) == 0) mine[e] += __popc(same);
+        __syncwarp();
+    }
+    __syncthreads();
+    for (int e = tid; e < E; e += SORT_THREADS) {
+        int32_t run = 0;
+#pragma unroll
+        for (int w = 0; w < SORT_WARPS; ++w) {
+            const int32_t c = cnt[w * E + e];
+            cnt[w * E + e] = run;
+            run += c;
+        }
+        total[e] = run;
+    }
+    if constexpr (CTAS > 1) cluster_barrier();
+    else __syncthreads();
+    // E <= 1024 = SORT_THREADS: thread e owns expert e
+    int32_t all = 0, before = 0;
+    if (tid < E) {
+#pragma unroll
+        for (int r = 0; r < CTAS; ++r) {
+            const int32_t c = CTAS > 1 ? ld_cluster_s32(&total[tid], (uint32_t)r) : total[tid];
+            if (r < (int)rank) before += c;
+            all += c;
+        }
+    }
+    int32_t scan = all;
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+        const int32_t up = __shfl_up_sync(0xffffffffu, scan, d);
+        if (lane >= d) scan += up;
+    }
+    if (lane == 31) warp_sum[warp] = scan;
+    __syncthreads();
+    int32_t below = lane < warp ? warp_sum[lane] : 0;
+    below = __reduce_add_sync(0xffffffffu, below);
+    const int32_t start = below + scan - all;       // first row of expert tid
+    if (rank == 0) {
+        if (tid < E) offsets[tid] = start;
+        if (tid == E - 1) offsets[E] = start + all;
+    }
+    if (tid < E) {
+        const int32_t base = start + before;
+#pragma unroll
+        for (int w = 0; w < SORT_WARPS; ++w) cnt[w * E + tid] += base;
+    }
+    __syncthreads();
+    for (int64_t i = first; i < end; i += 32) {
+        const int e = expert_of(ids, i + lane, end, E);
+        const uint32_t same = __match_any_sync(0xffffffffu, e);
+        const uint32_t lower = same & ((1u << lane) - 1);
+        const int32_t at = e >= 0 ? mine[e] + __popc(lower) : -1;
+        __syncwarp();
+        if (e >= 0 && lower == 0) mine[e] += __popc(same);
+        __syncwarp();
+        if (i + lane < end) pos[i + lane] = at;
+    }
+    if constexpr (CTAS > 1) cluster_barrier();      // no CTA leaves while its totals may be read
+}
+
+size_t sort_smem_bytes(int E) { return (size_t)(SORT_WARPS + 1) * E * sizeof(int32_t); }
+
+template <typename Id>
+int launch_sort(const Id* ids, int64_t n, int E, int32_t* pos, int32_t* offsets, cudaStream_t st)
+{
+    const size_t smem = sort_smem_bytes(E);
+    if (n <= 4096) {
+        expert_sort_kernel<Id, 1><<<1, SORT_THREADS, smem, st>>>(ids, n, E, pos, offsets);
+        return check_launch("expert_sort");
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(SORT_CLUSTER);
+    cfg.blockDim = dim3(SORT_THREADS);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = SORT_CLUSTER;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    cudaError_t e = cudaLaunchKernelEx(&cfg, expert_sort_kernel<Id, SORT_CLUSTER>, ids, n, E, pos, offsets);
+    if (e != cudaSuccess) return fail(WUSH_ERR_CUDA, "expert_sort: launch failed: %s", cudaGetErrorString(e));
+    return WUSH_OK;
+}
+
+// ---- moves -----------------------------------------------------------------------------------------------------------------
+// V: what one thread moves at once (16 bytes where the row length and the pointers allow it, else one element).
+template <typename T> __device__ __forceinline__ float to_f32(T v);
+template <> __device__ __forceinline__ float to_f32(float v) { return v; }
+template <> __device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+template <> __device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T> __device__ __forceinline__ T from_f32(float v);
+template <> __device__ __forceinline__ float from_f32(float v) { return v; }
+template <> __device__ __forceinline__ __half from_f32(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f32(float v) { return __float2bfloat16_rn(v); }
+
+template <typename T, int N> struct alignas(sizeof(T) * N) Pack { T v[N]; };
+
+// Row of an entry, or -1.  Positions come from the caller: one outside the rows counts as no row, so that nothing is
+// read or written out of range.
+__device__ __forceinline__ int64_t row_of(const int32_t* pos, int64_t i, int64_t total)
+{
+    const int64_t at = pos[i];
+    return at < total ? at : -1;
+}
+
+// Zero rows behind the last entry, dealt to the blocks.
+template <typename P>
+__device__ __forceinline__ void zero_tail(P* rows, int64_t n_vec, int64_t used, int64_t total, int block, int blocks, int tid, int threads)
+{
+    P z;
+    memset(&z, 0, sizeof(z));
+    for (int64_t r = (used > 0 ? used : 0) + block; r < total; r += blocks)
+        for (int64_t v = tid; v < n_vec; v += threads) rows[r * n_vec + v] = z;
+}
+
+template <typename T, int N>
+__global__ void __launch_bounds__(256) expert_gather_kernel(const Pack<T, N>* __restrict__ x, int64_t tokens, int n_vec,
+                                                            const int32_t* __restrict__ pos, int k,
+                                                            const int32_t* __restrict__ n_used, Pack<T, N>* __restrict__ rows)
+{
+    pdl_wait();
+    pdl_launch_dependents();
+    const int64_t t = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
+    if (t < tokens) {
+        for (int v = threadIdx.x; v < n_vec; v += blockDim.x) {
+            const Pack<T, N> p = x[t * n_vec + v];
+            for (int j = 0; j < k; ++j) {
+                const int64_t at = row_of(pos, t * k + j, tokens * k);
+                if (at >= 0) rows[at * n_vec + v] = p;
+            }
+        }
+    }
+    zero_tail(rows, n_vec, *n_used, tokens * k, blockIdx.x, gridDim.x, threadIdx.y * blockDim.x + threadIdx.x, blockDim.x * blockDim.y);
+}
+
+template <typename T, int N>
+__global__ void __launch_bounds__(256) expert_combine_kernel(const Pack<T, N>* __restrict__ rows, int64_t tokens, int n_vec,
+                                                             const int32_t* __restrict__ pos, int k,
+                                                             const float* __restrict__ weights, Pack<T, N>* __restrict__ y)
+{
+    pdl_wait();
+    pdl_launch_dependents();
+    const int64_t t = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
+    if (t >= tokens) return;
+    constexpr int AT_ONCE = 8;                                  // rows in flight per thread
+    for (int v = threadIdx.x; v < n_vec; v += blockDim.x) {
+        float acc[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) acc[i] = 0.f;
+        for (int j0 = 0; j0 < k; j0 += AT_ONCE) {
+            Pack<T, N> p[AT_ONCE];
+            float w[AT_ONCE];
+            bool here[AT_ONCE];
+#pragma unroll
+            for (int j = 0; j < AT_ONCE; ++j) {
+                const int64_t at = j0 + j < k ? row_of(pos, t * k + j0 + j, tokens * k) : -1;
+                here[j] = at >= 0;
+                if (here[j]) {
+                    p[j] = rows[at * n_vec + v];
+                    w[j] = weights ? weights[t * k + j0 + j] : 1.f;
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < AT_ONCE; ++j)
+                if (here[j]) {
+#pragma unroll
+                    for (int i = 0; i < N; ++i) acc[i] = __fmaf_rn(w[j], to_f32<T>(p[j].v[i]), acc[i]);
+                }
+        }
+        Pack<T, N> o;
+#pragma unroll
+        for (int i = 0; i < N; ++i) o.v[i] = from_f32<T>(acc[i]);
+        y[t * n_vec + v] = o;
+    }
+}
+
+// One block per token: dy is read once per chunk of entries, the dot products end in a block sum in a fixed order.
+template <typename T, int N>
+__global__ void __launch_bounds__(256) expert_combine_grad_kernel(const Pack<T, N>* __restrict__ dy, const Pack<T, N>* __restrict__ rows,
+                                                                  int64_t tokens, int n_vec, const int32_t* __restrict__ pos, int k,
+                                                                  const float* __restrict__ weights,
+                                                                  const int32_t* __restrict__ n_used, Pack<T, N>* __restrict__ d_rows,
+                                                                  float* __restrict__ d_w)
+{
+    constexpr int AT_ONCE = 4;
+    __shared__ float part[AT_ONCE][8];
+    pdl_wait();
+    pdl_launch_dependents();
+    const int64_t t = blockIdx.x;
+    const int tid = threadIdx.x, warps = blockDim.x >> 5;
+    for (int j0 = 0; j0 < k; j0 += AT_ONCE) {
+        int64_t at[AT_ONCE];
+        float w[AT_ONCE], dot[AT_ONCE];
+#pragma unroll
+        for (int j = 0; j < AT_ONCE; ++j) {
+            at[j] = j0 + j < k ? row_of(pos, t * k + j0 + j, tokens * k) : -1;
+            w[j] = at[j] >= 0 ? weights[t * k + j0 + j] : 0.f;
+            dot[j] = 0.f;
+        }
+        for (int v = tid; v < n_vec; v += blockDim.x) {
+            const Pack<T, N> g = dy[t * n_vec + v];
+            Pack<T, N> p[AT_ONCE];
+#pragma unroll
+            for (int j = 0; j < AT_ONCE; ++j)
+                if (at[j] >= 0) p[j] = rows[at[j] * n_vec + v];
+#pragma unroll
+            for (int j = 0; j < AT_ONCE; ++j)
+                if (at[j] >= 0) {
+                    Pack<T, N> o;
+#pragma unroll
+                    for (int i = 0; i < N; ++i) {
+                        const float gi = to_f32<T>(g.v[i]);
+                        dot[j] = __fmaf_rn(gi, to_f32<T>(p[j].v[i]), dot[j]);
+                        o.v[i] = from_f32<T>(__fmul_rn(w[j], gi));
+                    }
+                    d_rows[at[j] * n_vec + v] = o;
+                }
+        }
+#pragma unroll
+        for (int j = 0; j < AT_ONCE; ++j) {
+#pragma unroll
+            for (int d = 16; d; d >>= 1) dot[j] += __shfl_xor_sync(0xffffffffu, dot[j], d);
+            if ((tid & 31) == 0) part[j][tid >> 5] = dot[j];
+        }
+        __syncthreads();
+        if (tid < AT_ONCE && j0 + tid < k) {
+            float sum = 0.f;
+            for (int i = 0; i < warps; ++i) sum += part[tid][i];
+            d_w[t * k + j0 + tid] = sum;
+        }
+        __syncthreads();
+    }
+    zero_tail(d_rows, n_vec, *n_used, tokens * k, blockIdx.x, gridDim.x, tid, blockDim.x);
+}
+
+// Threads along a row: of 32, 64, 128, 256 the count that leaves the fewest idle in the last step, the largest of equals.
+int threads_along(int64_t n_vec)
+{
+    int best = 32;
+    int64_t cost = (n_vec + 31) / 32 * 32;
+    for (int t = 64; t <= 256; t *= 2) {
+        const int64_t c = (n_vec + t - 1) / t * t;
+        if (c <= cost) { best = t; cost = c; }
+    }
+    return best;
+}
+
+// Calls f with a Pack type: 16 bytes if the rows and the pointers allow it, else one element.
+template <typename T, typename F>
+int with_pack(bool wide, F f)
+{
+    if (wide) return f(Pack<T, 16 / sizeof(T)>{});
+    return f(Pack<T, 1>{});
+}
+template <typename F>
+int with_type(int dtype, bool wide, F f)
+{
+    switch (dtype) {
+        case WUSH_BF16: return with_pack<__nv_bfloat16>(wide, f);
+        case WUSH_F16: return with_pack<__half>(wide, f);
+        default: return with_pack<float>(wide, f);
+    }
+}
+template <typename T, int N> constexpr int pack_size(const Pack<T, N>&) { return N; }
+int64_t dtype_bytes(int dtype) { return dtype == WUSH_F32 ? 4 : 2; }
+bool wide_rows(int dtype, int64_t H, const void* a, const void* b, const void* c)
+{
+    return (H * dtype_bytes(dtype)) % 16 == 0 && aligned16(a) && aligned16(b) && aligned16(c);
+}
+bool element_aligned(int dtype, const void* p) { return (reinterpret_cast<uintptr_t>(p) & (uintptr_t)(dtype_bytes(dtype) - 1)) == 0; }
+
+template <typename T, int N>
+int launch_gather(Pack<T, N>, const void* x, int64_t tokens, int64_t H, const int32_t* pos, int k, const int32_t* n_used, void* rows,
+                  cudaStream_t st)
+{
+    const int n_vec = (int)(H / N), tx = threads_along(n_vec), ty = 256 / tx;
+    expert_gather_kernel<T, N><<<(unsigned)((tokens + ty - 1) / ty), dim3(tx, ty), 0, st>>>((const Pack<T, N>*)x, tokens, n_vec, pos, k,
+                                                                                        n_used, (Pack<T, N>*)rows);
+    return check_launch("expert_gather");
+}
+template <typename T, int N>
+int launch_combine(Pack<T, N>, const void* rows, int64_t tokens, int64_t H, const int32_t* pos, int k, const float* weights, void* y,
+                   bool dependent, cudaStream_t st)
+{
+    const int n_vec = (int)(H / N), tx = threads_along(n_vec), ty = 256 / tx;
+    const dim3 grid((unsigned)((tokens + ty - 1) / ty)), block(tx, ty);
+    if (dependent) {
+        cudaError_t e = launch_dependent(expert_combine_kernel<T, N>, grid, block, 0, st, (const Pack<T, N>*)rows, tokens, n_vec, pos, k,
+                                         weights, (Pack<T, N>*)y);
+        if (e != cudaSuccess) return fail(WUSH_ERR_CUDA, "expert_combine: launch failed: %s", cudaGetErrorString(e));
+        return WUSH_OK;
+    }
+    expert_combine_kernel<T, N><<<grid, block, 0, st>>>((const Pack<T, N>*)rows, tokens, n_vec, pos, k, weights, (Pack<T, N>*)y);
+    return check_launch("expert_combine");
+}
+template <typename T, int N>
+int launch_grad(Pack<T, N>, const void* dy, const void* rows, int64_t tokens, int64_t H, const int32_t* pos, int k, const float* weights,
+                const int32_t* n_used, void* d_rows, float* d_w, cudaStream_t st)
+{
+    const int n_vec = (int)(H / N);
+    expert_combine_grad_kernel<T, N><<<(unsigned)tokens, threads_along(n_vec), 0, st>>>(
+        (const Pack<T, N>*)dy, (const Pack<T, N>*)rows, tokens, n_vec, pos, k, weights, n_used, (Pack<T, N>*)d_rows, d_w);
+    return check_launch("expert_combine_grad");
+}
+
+int check_moves(const char* op, int dtype, int64_t tokens, int64_t H)
+{
+    if (dtype < WUSH_BF16 || dtype > WUSH_F32) return fail(WUSH_ERR_INVALID_ARGUMENT, "%s: unknown dtype %d", op, dtype);
+    if (tokens < 0 || H < 1 || H > (1 << 30)) return fail(WUSH_ERR_INVALID_ARGUMENT, "%s: rows of 1..2^30 elements (got %lld)", op, (long long)H);
+    return WUSH_OK;
+}
+
+}  // namespace
+
+int expert_order_set_attributes()
+{
+    const int most = (int)sort_smem_bytes(WUSH_EXPERT_MAX);
+    cudaError_t e = cudaFuncSetAttribute(expert_sort_kernel<int32_t, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(expert_sort_kernel<int64_t, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+    if (e == cudaSuccess)
+        e = cudaFuncSetAttribute(expert_sort_kernel<int32_t, SORT_CLUSTER>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+    if (e == cudaSuccess)
+        e = cudaFuncSetAttribute(expert_sort_kernel<int64_t, SORT_CLUSTER>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+    if (e != cudaSuccess) return fail(WUSH_ERR_CUDA, "expert_sort: cudaFuncSetAttribute failed: %s", cudaGetErrorString(e));
+    return WUSH_OK;
+}
+
+int expert_sort_launch(const void* ids, int id_bytes, int64_t n, int n_experts, int32_t* pos, int32_t* offsets, cudaStream_t st)
+{
+    if (id_bytes == 8) return launch_sort<int64_t>((const int64_t*)ids, n, n_experts, pos, offsets, st);
+    return launch_sort<int32_t>((const int32_t*)ids, n, n_experts, pos, offsets, st);
+}
+
+int expert_combine_launch(const void* rows, int dtype, int64_t tokens, int64_t H, const int32_t* pos, int k, const float* weights,
+                          void* y, bool dependent, cudaStream_t st)
+{
+    return with_type(dtype, wide_rows(dtype, H, rows, y, y),
+                     [&](auto p) { return launch_combine(p, rows, tokens, H, pos, k, weights, y, dependent, st); });
+}
+
+}  // namespace wush
+
+WUSH_API int wush_expert_sort(const void* ids, int id_bytes, int64_t tokens, int64_t k, int64_t n_experts, int32_t* pos, int32_t* offsets,
+                              void* stream)
+{
+    using namespace wush;
+    WUSH_REQUIRE(id_bytes == 4 || id_bytes == 8, "expert_sort: ids are 4 or 8 bytes wide (got %d)", id_bytes);
+    if (int e = check_entries("expert_sort", tokens, k, n_experts)) return e;
+    WUSH_REQUIRE(offsets && (tokens == 0 || (ids && pos)), "expert_sort: null pointer");
+    WUSH_REQUIRE((reinterpret_cast<uintptr_t>(ids) & (uintptr_t)(id_bytes - 1)) == 0 && aligned4(pos) && aligned4(offsets),
+                 "expert_sort: misaligned pointer");
+    if (int e = ensure_init()) return e;
+    return expert_sort_launch(ids, id_bytes, tokens * k, (int)n_experts, pos, offsets, (cudaStream_t)stream);
+}
+
+WUSH_API int wush_expert_gather(const void* x, int dtype, int64_t tokens, int64_t H, const int32_t* pos, int64_t k, const int32_t* offsets,
+                                int64_t n_experts, void* rows, void* stream)
+{
+    using namespace wush;
+    if (int e = check_moves("expert_gather", dtype, tokens, H)) return e;
+    if (int e = check_entries("expert_gather", tokens, k, n_experts)) return e;
+    if (tokens == 0) return WUSH_OK;
+    WUSH_REQUIRE(x && pos && offsets && rows, "expert_gather: null pointer");
+    WUSH_REQUIRE(element_aligned(dtype, x) && element_aligned(dtype, rows) && aligned4(pos) && aligned4(offsets),
+                 "expert_gather: misaligned pointer");
+    if (int e = ensure_init()) return e;
+    return with_type(dtype, wide_rows(dtype, H, x, rows, rows), [&](auto p) {
+        return launch_gather(p, x, tokens, H, pos, (int)k, offsets + n_experts, rows, (cudaStream_t)stream);
+    });
+}
+
+WUSH_API int wush_expert_combine(const void* rows, int dtype, int64_t tokens, int64_t H, const int32_t* pos, int64_t k,
+                                 const float* weights, void* y, void* stream)
+{
+    using namespace wush;
+    if (int e = check_moves("expert_combine", dtype, tokens, H)) return e;
+    if (int e = check_entries("expert_combine", tokens, k, 1)) return e;
+    if (tokens == 0) return WUSH_OK;
+    WUSH_REQUIRE(rows && pos && y, "expert_combine: null pointer");
+    WUSH_REQUIRE(element_aligned(dtype, rows) && element_aligned(dtype, y) && aligned4(pos) && aligned4(weights),
+                 "expert_combine: misaligned pointer");
+    if (int e = ensure_init()) return e;
+    return expert_combine_launch(rows, dtype, tokens, H, pos, (int)k, weights, y, false, (cudaStream_t)stream);
+}
+
+WUSH_API int wush_expert_combine_grad(const void* dy, const void* rows, int dtype, int64_t tokens, int64_t H, const int32_t* pos, int64_t k,
+                                      const int32_t* offsets, int64_t n_experts, const float* weights, void* d_rows, float* d_weights,
+                                      void* stream)
+{
+    using namespace wush;
+    if (int e = check_moves("expert_combine_grad", dtype, tokens, H)) return e;
+    if (int e = check_entries("expert_combine_grad", tokens, k, n_experts)) return e;
+    if (tokens == 0) return WUSH_OK;
+    WUSH_REQUIRE(dy && rows && pos && offsets && weights && d_rows && d_weights, "expert_combine_grad: null pointer");
+    WUSH_REQUIRE(element_aligned(dtype, dy) && element_aligned(dtype, rows) && element_aligned(dtype, d_rows) && aligned4(pos) &&
+                     aligned4(offsets) && aligned4(weights) && aligned4(d_weights),
+                 "expert_combine_grad: misaligned pointer");
+    if (int e = ensure_init()) return e;
+    return with_type(dtype, wide_rows(dtype, H, dy, rows, d_rows), [&](auto p) {
+        return launch_grad(p, dy, rows, tokens, H, pos, (int)k, weights, offsets + n_experts, d_rows, d_weights, (cudaStream_t)stream);
+    });
+}

@@ -543,20 +543,22 @@ int stream_partials(const uint8_t* xq, const uint8_t* wq, int64_t M, int64_t N, 
 
 }  // namespace wush
 
-namespace wush { int static_scratch_take_error(int* word); }
+namespace wush { int static_scratch_take_error(int* word); int w8a8_take_error(int* word); }
 
 // Bits 0-7: role code of a streaming (decode) kernel whose wait ran out; bits 8-15: role code left by a
-// kernel of wush_w4a4_gemm_static_scratch (whose scratch, unlike a caller's, cannot be inspected from outside).
+// kernel of wush_w4a4_gemm_static_scratch (whose scratch, unlike a caller's, cannot be inspected from outside);
+// bits 16-23: role code left by a kernel of the 8-bit products.
 WUSH_API int wush_device_flag(int* flag)
 {
     using namespace wush;
     if (int e = ensure_init()) return e;
     WUSH_REQUIRE(flag, "device_flag: null pointer");
-    int zero = 0, stream_word = 0, static_word = 0;
+    int zero = 0, stream_word = 0, static_word = 0, w8a8_word = 0;
     cudaError_t e = cudaMemcpyFromSymbol(&stream_word, g_device_flag, sizeof(int));
     if (e == cudaSuccess) e = cudaMemcpyToSymbol(g_device_flag, &zero, sizeof(int));
     if (e != cudaSuccess) return fail(WUSH_ERR_CUDA, "device_flag: %s", cudaGetErrorString(e));
     if (int s = static_scratch_take_error(&static_word)) return s;
-    *flag = (stream_word & 0xff) | ((static_word & 0xff) << 8);
+    if (int s = w8a8_take_error(&w8a8_word)) return s;
+    *flag = (stream_word & 0xff) | ((static_word & 0xff) << 8) | ((w8a8_word & 0xff) << 16);
     return WUSH_OK;
 }

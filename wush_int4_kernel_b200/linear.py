@@ -84,6 +84,35 @@ class W4A4Linear:
         return W4A4Linear(self.t.to(device), self.wq.to(device), self.ws.to(device))
 
 
+@dataclass
+class W8A8Linear:
+    """y = W8A8(x) + bias: one scale per activation row and per output channel, for layers that do not bear 4 bits.
+    Takes bf16 or fp16 activations and returns their type; the quantiser and the product are one call."""
+    wq: torch.Tensor                       # (N, K) int8
+    ws: torch.Tensor                       # (N) fp32
+    bias: torch.Tensor | None = None       # (N) fp32
+
+    @classmethod
+    def from_weight(cls, weight: torch.Tensor, bias: torch.Tensor | None = None) -> "W8A8Linear":
+        """Quantises a (N, K) CUDA weight (bf16, fp16 or fp32)."""
+        wq, ws = _ops().quant_int8(weight.contiguous())
+        return cls(wq, ws, None if bias is None else bias.float().contiguous())
+
+    @property
+    def in_features(self) -> int:
+        return self.wq.shape[1]
+
+    @property
+    def out_features(self) -> int:
+        return self.wq.shape[0]
+
+    def __call__(self, x: torch.Tensor) -> torch.Tensor:
+        return _ops().w8a8_linear(x.contiguous(), self.wq, self.ws, self.bias)
+
+    def to(self, device) -> "W8A8Linear":
+        return W8A8Linear(self.wq.to(device), self.ws.to(device), None if self.bias is None else self.bias.to(device))
+
+
 class ColumnParallelW4A4Linear:
     """Rank ``rank`` of ``world`` holds output columns ``shard_bounds(N, world, rank, multiple)``."""
 
