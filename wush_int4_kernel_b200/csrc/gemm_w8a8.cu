@@ -371,6 +371,264 @@ __global__ void __launch_bounds__(THREADS, 2) w8a8_small_kernel(const __grid_con
     if (warp == 1) tc::tmem_dealloc(tmem, C::COLS);
 }
 
+// ---- many tokens: CTA pairs -------------------------------------------------------------------------------------------------
+// 256 channels x up to 256 tokens per pair of CTAs (cta_group::2): each CTA holds 128 weight rows and half of the token rows
+// of a stage, two accumulators rotate in tensor memory so the epilogue of a tile runs under the MMAs of the next, and the
+// pairs are persistent.  The token count of a tile is a multiple of 32 chosen per expert (its rows in equal tiles), so a
+// ragged expert costs MMAs for at most 31 rows that do not exist, not for a full tile.
+constexpr int PAIR_TOKENS = 256, PAIR_STAGES = 6, PAIR_ACC = 2;
+constexpr int PAIR_STAGE = 2 * A_BYTES;                  // 128 weight rows and up to 128 token rows
+constexpr int PAIR_SX = PAIR_STAGES * PAIR_STAGE;        // token scales of two tiles
+constexpr int PAIR_TABLE = PAIR_SX + 2 * PAIR_TOKENS * 4;
+constexpr int PAIR_TABLE_BYTES = 2 * (WUSH_EXPERT_MAX + 2) * 4;
+constexpr int PAIR_BARS = PAIR_TABLE + PAIR_TABLE_BYTES;
+constexpr int PAIR_SMEM = PAIR_BARS + (2 * PAIR_STAGES + 2 * PAIR_ACC + 1) * 8 + 16 + 1024;
+static_assert(PAIR_BARS % 8 == 0, "barriers are 8-byte aligned");
+
+struct PairMaps {
+    CUtensorMap w;
+    CUtensorMap x[3];            // boxes of 32, 64, 128 token rows
+};
+
+__device__ __forceinline__ void tma_load_4d_pair(void* dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int c2, int c3)
+{
+    asm volatile(
+        "cp.async.bulk.tensor.4d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(
+            tc::smem_u32(dst)),
+        "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+        : "memory");
+}
+
+struct Tile {
+    int expert, ct, n_rows, nt;  // nt: token columns of the tile, a multiple of 32
+    int64_t row0;
+};
+
+// Token tiles of `count` rows: as few as possible, of equal size.  (tiles - 1) * nt < count, because nt <= 256.
+__host__ __device__ __forceinline__ int token_tiles(int64_t count) { return (int)((count + PAIR_TOKENS - 1) / PAIR_TOKENS); }
+__device__ __forceinline__ int tile_width(int64_t count, int tiles) { return (int)(((count + tiles - 1) / tiles + 31) & ~31ll); }
+
+// Tile t in the order in which the pairs take them.  Inside a group of token tiles the tokens run fastest, so tiles that
+// run together share weight rows and one wave's weights are read from HBM once.  Groups: the experts, or, with one
+// expert, bands of `band` token tiles whose activations stay in L2 while the band sweeps the channels.
+struct TileOrder {
+    const Params& p;
+    const int32_t* first;        // shared memory: first tile of each expert
+    const int32_t* row;          // shared memory: first row of each expert
+    int band, e;
+
+    __device__ __forceinline__ Tile at(int t)
+    {
+        Tile r;
+        int64_t count, start;
+        int tok;
+        if (first) {
+            while (t >= first[e + 1]) ++e;
+            start = row[e];
+            count = row[e + 1] - row[e];
+            const int tiles = token_tiles(count), local = t - first[e];
+            tok = local % tiles;
+            r.ct = local / tiles;
+            r.nt = tile_width(count, tiles);
+        } else {
+            start = 0;
+            count = p.rows;
+            const int tiles = token_tiles(count), b = t / (band * p.tiles_c), local = t - b * band * p.tiles_c;
+            const int here = min(band, tiles - b * band);
+            tok = b * band + local % here;
+            r.ct = local / here;
+            r.nt = tile_width(count, tiles);
+        }
+        r.expert = e;
+        r.row0 = start + (int64_t)tok * r.nt;
+        r.n_rows = (int)min((int64_t)r.nt, count - (int64_t)tok * r.nt);
+        return r;
+    }
+};
+
+template <bool GATED>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
+w8a8_pair_kernel(const __grid_constant__ PairMaps maps, const Params p, int band)
+{
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    float* sx_s = reinterpret_cast<float*>(smem + PAIR_SX);
+    int32_t* first_s = reinterpret_cast<int32_t*>(smem + PAIR_TABLE);
+    int32_t* row_s = first_s + WUSH_EXPERT_MAX + 2;
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + PAIR_BARS);     // used in rank 0: both CTAs' stage data landed
+    uint64_t* empty = full + PAIR_STAGES;                                // per CTA: the MMAs reading this stage are done
+    uint64_t* acc_full = empty + PAIR_STAGES;                            // per CTA: a tile's sums are complete
+    uint64_t* acc_empty = acc_full + PAIR_ACC;                           // used in rank 0: both CTAs' epilogues have read them
+    uint64_t* done_bar = acc_empty + PAIR_ACC;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done_bar + 1);
+
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const uint32_t rank = tc::cluster_ctarank();
+    const int pair = blockIdx.x >> 1, n_pairs = gridDim.x >> 1;
+
+    pdl_wait();
+    pdl_launch_dependents();
+    if (tid == 0) {
+        for (int i = 0; i < PAIR_STAGES; ++i) { tc::mbar_init(&full[i], 1); tc::mbar_init(&empty[i], 1); }
+        for (int i = 0; i < PAIR_ACC; ++i) { tc::mbar_init(&acc_full[i], 1); tc::mbar_init(&acc_empty[i], 8); }
+        tc::mbar_init(done_bar, 1);
+        tc::mbar_fence_init();
+    }
+    if (warp == 1) {
+        tc::tmem_alloc_pair(tmem_slot, 512);
+        tc::tmem_relinquish_pair();
+    }
+    if (warp == 0 && p.offsets) {                        // the table of tiles
+        int before = 0;
+        for (int e0 = 0; e0 < p.experts; e0 += 32) {
+            const int e = e0 + lane;
+            int64_t a = 0, b = 0;
+            if (e < p.experts) { a = first_row(p, e); b = first_row(p, e + 1); }
+            const int tiles = b > a ? token_tiles(b - a) * p.tiles_c : 0;
+            int scan = tiles;
+#pragma unroll
+            for (int d = 1; d < 32; d *= 2) {
+                const int up = __shfl_up_sync(0xffffffffu, scan, d);
+                if (lane >= d) scan += up;
+            }
+            if (e < p.experts) {
+                first_s[e] = before + scan - tiles;
+                row_s[e] = (int32_t)a;
+                if (e == p.experts - 1) { first_s[e + 1] = before + scan; row_s[e + 1] = (int32_t)b; }
+            }
+            before += __shfl_sync(0xffffffffu, scan, 31);
+        }
+    }
+    tc::tc_fence_before();
+    __syncthreads();
+    tc::cluster_sync_all();                              // the other CTA's barriers exist before anything targets them
+    tc::tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    const int n_tiles = p.offsets ? first_s[p.experts] : token_tiles(p.rows) * p.tiles_c;
+    TileOrder order = {p, p.offsets ? first_s : nullptr, row_s, band, 0};
+    const int k_steps = (p.K + 127) / 128;
+    constexpr int WIDTH = GATED ? 64 : 128;              // channels of the result per CTA
+
+    if (warp == 0) {
+        if (lane == 0) {
+            uint32_t slot = 0, phase = 0;
+            int issued = 0;
+            bool ok = true;
+            for (int t = pair; t < n_tiles && ok; t += n_pairs) {
+                const Tile tile = order.at(t);
+                const int half = tile.nt / 2, c0 = tile.ct * 2 * WIDTH + (int)rank * WIDTH;
+                const int m = half <= 32 ? 0 : half <= 64 ? 1 : 2, row = (int)tile.row0 + (int)rank * half;
+                const uint32_t bytes = 2 * (A_BYTES + (32 << m) * 128);          // of both CTAs
+                const CUtensorMap* mx = &maps.x[m];
+                for (int ks = 0; ks < k_steps; ++ks) {
+                    if (!tc::mbar_wait(&empty[slot], phase ^ 1)) { ok = false; break; }
+                    uint8_t* st = smem + slot * PAIR_STAGE;
+                    const uint32_t bar = tc::map_to_rank(&full[slot], 0);
+                    if (rank == 0) tc::mbar_expect_tx(&full[slot], bytes);
+                    tma_load_4d_pair(st, &maps.w, bar, ks * 128, 0, c0, tile.expert);
+                    tc::tma_load_2d_pair(st + A_BYTES, mx, bar, ks * 128, row);
+                    ++issued;
+                    if (++slot == PAIR_STAGES) { slot = 0; phase ^= 1; }
+                }
+            }
+            if (!ok) {
+                atomicExch(&g_w8a8_err, 1);
+                // Copies already issued must land before this CTA's shared memory is given back; rank 0 can watch its
+                // `full` barriers, rank 1, whose bytes are counted there, sleeps for as long.
+                if (rank == 0) {
+                    for (int i = 0; i < (issued < PAIR_STAGES ? issued : PAIR_STAGES); ++i)
+                        for (uint32_t spin = 0; spin < (1u << 16); ++spin)
+                            if (tc::mbar_try_wait(&full[i], 0) || tc::mbar_try_wait(&full[i], 1)) break;
+                } else {
+                    for (int i = 0; i < 64; ++i) __nanosleep(20000);
+                }
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0 && rank == 0) {
+            uint32_t slot = 0, phase = 0, ab = 0, aphase = 0;
+            bool ok = true;
+            for (int t = pair; t < n_tiles && ok; t += n_pairs) {
+                const Tile tile = order.at(t);
+                const uint32_t idesc = tc::idesc_i8_pair(tile.nt);
+                if (!tc::mbar_wait(&acc_empty[ab], aphase ^ 1)) { ok = false; break; }
+                tc::tc_fence_after();
+                for (int ks = 0; ks < k_steps; ++ks) {
+                    if (!tc::mbar_wait(&full[slot], phase)) { ok = false; break; }
+                    tc::tc_fence_after();
+                    const uint32_t sa = tc::smem_u32(smem + slot * PAIR_STAGE), sb = sa + A_BYTES;
+#pragma unroll
+                    for (int kk = 0; kk < 4; ++kk)
+                        tc::mma_i8_pair(tmem + ab * PAIR_TOKENS, desc_sw128(sa + kk * 32), desc_sw128(sb + kk * 32), idesc, (ks | kk) ? 1u : 0u);
+                    tc::mma_commit_pair(&empty[slot]);                           // frees the stage in both CTAs
+                    if (++slot == PAIR_STAGES) { slot = 0; phase ^= 1; }
+                }
+                if (!ok) break;
+                tc::mma_commit_pair(&acc_full[ab]);                              // both CTAs' epilogues may read
+                if (++ab == PAIR_ACC) { ab = 0; aphase ^= 1; }
+            }
+            if (!ok) atomicExch(&g_w8a8_err, 2);
+            tc::mma_commit_pair(done_bar);
+            for (uint32_t spin = 0; spin < WUSH_SPIN_LIMIT; ++spin)
+                if (tc::mbar_try_wait(done_bar, 0)) break;
+        }
+    } else {
+        const int quarter = warp & 3, c = quarter * 32 + lane;                   // tcgen05.ld: a warp reads lanes 32 * (warp % 4) ...
+        const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
+        if (p.offsets)                                                           // rows behind the last expert's
+            for (int64_t r = row_s[p.experts] + (int64_t)blockIdx.x; r < p.rows; r += gridDim.x)
+                for (int64_t i = tid - 64; i < p.N; i += THREADS - 64) {
+                    if constexpr (GATED) reinterpret_cast<float*>(p.y)[r * p.N + i] = 0.f;
+                    else reinterpret_cast<uint16_t*>(p.y)[r * p.N + i] = 0;
+                }
+        uint32_t ab = 0, aphase = 0;
+        bool ok = true;
+        for (int t = pair; t < n_tiles; t += n_pairs) {
+            const Tile tile = order.at(t);
+            Lane L;
+            L.row0 = tile.row0;
+            L.n_rows = tile.n_rows;
+            L.n = (int64_t)tile.ct * 2 * WIDTH + rank * WIDTH + (GATED ? c >> 1 : c);
+            L.sw = 0.f;
+            L.bias = 0.f;
+            if (L.n < p.N) {
+                L.sw = p.ws[(int64_t)tile.expert * (GATED ? 2 * p.N : p.N) + L.n + (GATED && (c & 1) ? p.N : 0)];
+                if (!GATED && p.bias) L.bias = p.bias[L.n];
+            }
+            float* sx = sx_s + ab * PAIR_TOKENS;
+            for (int i = tid - 64; i < tile.nt; i += THREADS - 64) sx[i] = i < tile.n_rows ? p.xs[tile.row0 + i] : 0.f;
+            asm volatile("bar.sync 1, 128;" ::: "memory");                       // the epilogue's own barrier
+            L.sx = sx;
+            if (ok) ok = __all_sync(0xffffffffu, tc::mbar_wait(&acc_full[ab], aphase));
+            tc::tc_fence_after();
+            const int chunks = ok ? tile.nt / 32 : 0;        // after a give-up: no more work, but every barrier of the warps
+#pragma unroll 1
+            for (int c0 = 0; c0 < chunks; ++c0) {
+                uint32_t v[32];
+                tc::tmem_ld32(tmem + lane_base + ab * PAIR_TOKENS + c0 * 32, v);
+                tc::tmem_ld_wait();
+                if (c0 == chunks - 1) {
+                    tc::tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) tc::mbar_arrive_cluster(tc::map_to_rank(&acc_empty[ab], 0));
+                }
+#pragma unroll
+                for (int j = 0; j < 32; j += 2)
+                    if (c0 * 32 + j < tile.n_rows) emit_pair<GATED>(p, L, c0 * 32 + j, v[j], v[j + 1]);
+            }
+            if (++ab == PAIR_ACC) { ab = 0; aphase ^= 1; }
+        }
+        if (!ok && lane == 0) atomicExch(&g_w8a8_err, 4);
+    }
+
+    // Neither CTA may leave while the other can still signal its barriers or while the shared MMA reads its shared memory,
+    // and the tensor memory is freed by both together.
+    tc::tc_fence_before();
+    __syncthreads();
+    tc::cluster_sync_all();
+    if (warp == 1) tc::tmem_dealloc_pair(tmem, 512);
+}
+
 // Weights (experts, 1 or 2, channels, K) and a box of 128 rows of 128 bytes; the order of the dimensions interleaves the two
 // halves of a gated layer.
 int make_weight_map(CUtensorMap* map, const W8A8Problem& p)
@@ -438,6 +696,68 @@ int set_small()
     return WUSH_OK;
 }
 
+int g_pairs_resident[64];        // per device: pairs of CTAs that can be resident at once
+
+template <bool GATED>
+int launch_pair(const W8A8Problem& w, Params p, bool dependent, cudaStream_t st)
+{
+    PairMaps maps;
+    if (int e = make_weight_map(&maps.w, w)) return e;
+    for (int i = 0; i < 3; ++i)
+        if (int e = make_token_map(&maps.x[i], w, 32 << i)) return e;
+    p.tiles_c = (int)((w.N + (GATED ? 127 : 255)) / (GATED ? 128 : 256));
+    int dev = 0;
+    cudaGetDevice(&dev);
+    const int resident = dev >= 0 && dev < 64 && g_pairs_resident[dev] > 0 ? g_pairs_resident[dev] : sm_count() / 2;
+    const int64_t most = ((int64_t)token_tiles(w.rows) + (w.offsets ? std::min(w.experts, w.rows) : 0)) * p.tiles_c;
+    if (most > 0x7fffffffll) return fail(WUSH_ERR_UNSUPPORTED, "w8a8: too many tiles (%lld)", (long long)most);
+    const int pairs = (int)std::min<int64_t>(most, resident);
+    // Band of token tiles whose activations take about a quarter of the L2 (32 MB).
+    const int band = (int)std::max<int64_t>(2, std::min<int64_t>(token_tiles(w.rows), (32ll << 20) / (PAIR_TOKENS * w.K)));
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(2 * pairs);
+    cfg.blockDim = dim3(THREADS);
+    cfg.dynamicSmemBytes = PAIR_SMEM;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = dependent ? 1 : 0;
+    cudaError_t e = cudaLaunchKernelEx(&cfg, w8a8_pair_kernel<GATED>, maps, p, band);
+    if (e != cudaSuccess) return fail(WUSH_ERR_CUDA, "w8a8: launch failed: %s", cudaGetErrorString(e));
+    return WUSH_OK;
+}
+
+int set_pair()
+{
+    cudaError_t e = cudaFuncSetAttribute(w8a8_pair_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, PAIR_SMEM);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(w8a8_pair_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, PAIR_SMEM);
+    if (e != cudaSuccess) return fail(WUSH_ERR_CUDA, "w8a8: cudaFuncSetAttribute failed: %s", cudaGetErrorString(e));
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev < 0 || dev >= 64) return WUSH_OK;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(sm_count() & ~1));
+    cfg.blockDim = dim3(THREADS);
+    cfg.dynamicSmemBytes = PAIR_SMEM;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int clusters = 0;
+    e = cudaOccupancyMaxActiveClusters(&clusters, w8a8_pair_kernel<false>, &cfg);
+    if (e != cudaSuccess || clusters <= 0) {
+        cudaGetLastError();
+        clusters = sm_count() / 2;
+    }
+    g_pairs_resident[dev] = clusters;
+    return WUSH_OK;
+}
+
 // CTAs along K of one tile: doubled while the launch has less than `want` CTAs and each keeps four stages of K or more.
 int pick_split(int64_t tiles, int k_steps, int nt, int64_t want)
 {
@@ -454,6 +774,7 @@ int w8a8_set_attributes()
     if (int s = set_small<16>()) return s;
     if (int s = set_small<32>()) return s;
     if (int s = set_small<64>()) return s;
+    if (int s = set_pair()) return s;
     return WUSH_OK;
 }
 
@@ -477,6 +798,7 @@ int w8a8_launch(const W8A8Problem& w, bool dependent, cudaStream_t st)
     const int width = w.gated ? 64 : 128;
     p.tiles_c = (int)((w.N + width - 1) / width);
     const int64_t groups = std::min(w.experts, w.rows), per = (w.rows + groups - 1) / groups;
+    if (per > 64) return w.gated ? launch_pair<true>(w, p, dependent, st) : launch_pair<false>(w, p, dependent, st);
     const int nt = per <= 16 ? 16 : per <= 32 ? 32 : 64;
     const int64_t slots = w.offsets ? w.rows / nt + groups : (w.rows + nt - 1) / nt;
     const int split = pick_split(slots * p.tiles_c, (int)((w.K + 127) / 128), nt, 8 * sm_count());
