@@ -242,9 +242,13 @@ typedef enum { WUSH_BF16 = 0, WUSH_F16 = 1, WUSH_F32 = 2 } wush_dtype;
 int wush_quant_int8(const void* x, int dtype, int64_t rows, int64_t K, int8_t* q, float* s, void* stream);
 
 /* y[m][n] = xs[m] * ws[n] * sum_k xq[m][k] * wq[n][k] (+ bias[n]), exact int32 sums, scales in fp32, one
- * rounding to `out_dtype` (WUSH_F16 or WUSH_BF16).  bias: N fp32 or NULL.  No scratch. */
+ * rounding to `out_dtype` (WUSH_F16 or WUSH_BF16).  bias: N fp32 or NULL.
+ * Scratch: wush_w8a8_gemm_workspace_bytes(M, 1), contents irrelevant, 16-byte aligned (may be NULL where that
+ * is 0); calls that may run at the same time need their own. */
+size_t wush_w8a8_gemm_workspace_bytes(int64_t M, int64_t experts);
 int wush_w8a8_gemm(const int8_t* xq, const float* xs, const int8_t* wq, const float* ws, const float* bias,
-                   int64_t M, int64_t N, int64_t K, void* y, int out_dtype, void* stream);
+                   int64_t M, int64_t N, int64_t K, void* y, int out_dtype, void* workspace, size_t workspace_bytes,
+                   void* stream);
 
 /* The two in one call: quantise x (M, K) of `dtype` (WUSH_F16 or WUSH_BF16) into the workspace, then the
  * product, whose kernel fetches its first weights while the quantiser runs.  y has the type of x. */
@@ -280,11 +284,14 @@ int wush_expert_combine_grad(const void* dy, const void* rows, int dtype, int64_
  * (wq (experts, N, K), ws (experts, N)); rows from offsets[experts] on become zero.
  *   gemm   as wush_w8a8_gemm without bias
  *   gated  wq (experts, 2 * I, K), the I gate channels first: h[m][i] = silu(g) * u in fp32 (rows, I), with g and
- *          u the products of channels i and I + i.  The result keeps fp32: it is what the next quantiser reads */
+ *          u the products of channels i and I + i.  The result keeps fp32: it is what the next quantiser reads
+ * Scratch: wush_w8a8_gemm_workspace_bytes(rows, experts), as for wush_w8a8_gemm. */
 int wush_w8a8_grouped_gemm(const int8_t* xq, const float* xs, const int8_t* wq, const float* ws, const int32_t* offsets,
-                           int64_t rows, int64_t experts, int64_t N, int64_t K, void* y, int out_dtype, void* stream);
+                           int64_t rows, int64_t experts, int64_t N, int64_t K, void* y, int out_dtype, void* workspace,
+                           size_t workspace_bytes, void* stream);
 int wush_w8a8_grouped_gated(const int8_t* xq, const float* xs, const int8_t* wq, const float* ws, const int32_t* offsets,
-                            int64_t rows, int64_t experts, int64_t I, int64_t K, float* h, void* stream);
+                            int64_t rows, int64_t experts, int64_t I, int64_t K, float* h, void* workspace, size_t workspace_bytes,
+                            void* stream);
 
 /* The whole block: sort, gather + quantise, gated product, quantise, product, weighted sum.
  * x, y: (tokens, H) of `dtype` (WUSH_F16 or WUSH_BF16); weights (tokens, k) fp32; w13q (experts, 2 * I, H),

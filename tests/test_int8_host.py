@@ -33,13 +33,15 @@ def test_quant_int8_refusals(lib, args):
 ])
 def test_w8a8_gemm_refusals(lib, change):
     a = dict(xq=P, xs=P, wq=P, ws=P, bias=None, M=4, N=64, K=64, y=P, out=capi.F16) | change
-    assert lib.wush_w8a8_gemm(a["xq"], a["xs"], a["wq"], a["ws"], a["bias"], a["M"], a["N"], a["K"], a["y"], a["out"], None) == BAD
+    assert lib.wush_w8a8_gemm(a["xq"], a["xs"], a["wq"], a["ws"], a["bias"], a["M"], a["N"], a["K"], a["y"], a["out"], None, 0,
+                              None) == BAD
 
 
 def test_w8a8_empty_is_fine(lib):
-    assert lib.wush_w8a8_gemm(None, None, None, None, None, 0, 64, 64, None, capi.F16, None) == 0
-    assert lib.wush_w8a8_gemm(None, None, None, None, None, 4, 0, 64, None, capi.F16, None) == 0
+    assert lib.wush_w8a8_gemm(None, None, None, None, None, 0, 64, 64, None, capi.F16, None, 0, None) == 0
+    assert lib.wush_w8a8_gemm(None, None, None, None, None, 4, 0, 64, None, capi.F16, None, 0, None) == 0
     assert lib.wush_quant_int8(None, capi.BF16, 0, 64, None, None, None) == 0
+    assert lib.wush_w8a8_gemm_workspace_bytes(0, 1) == 0 == lib.wush_w8a8_gemm_workspace_bytes(5, 0)
     assert lib.wush_w8a8_linear_workspace_bytes(0, 64) == 0 == lib.wush_w8a8_linear_workspace_bytes(4, 0)
     assert lib.wush_w8a8_expert_ffn_workspace_bytes(0, 64, 64, 4, 2) == 0
 
@@ -84,8 +86,8 @@ def test_expert_gather_quant_needs_sixteen(lib):
 @pytest.mark.parametrize("change", [dict(K=40), dict(E=0), dict(E=capi.EXPERT_MAX + 1), dict(off=None), dict(wq=P + 4), dict(rows=-1)])
 def test_grouped_refusals(lib, change):
     a = dict(wq=P, off=P, rows=8, E=4, N=32, K=64) | change
-    assert lib.wush_w8a8_grouped_gemm(P, P, a["wq"], P, a["off"], a["rows"], a["E"], a["N"], a["K"], P, capi.F16, None) == BAD
-    assert lib.wush_w8a8_grouped_gated(P, P, a["wq"], P, a["off"], a["rows"], a["E"], a["N"], a["K"], P, None) == BAD
+    assert lib.wush_w8a8_grouped_gemm(P, P, a["wq"], P, a["off"], a["rows"], a["E"], a["N"], a["K"], P, capi.F16, None, 0, None) == BAD
+    assert lib.wush_w8a8_grouped_gated(P, P, a["wq"], P, a["off"], a["rows"], a["E"], a["N"], a["K"], P, None, 0, None) == BAD
 
 
 def test_expert_ffn_refusals(lib):

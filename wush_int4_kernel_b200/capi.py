@@ -41,7 +41,8 @@ SIGNATURES = {
     "wush_quant_int4_tensor_scale": (_int, [_vp, _i64, _f32, _vp, _vp, _vp]),
     "wush_w4a4_gemm_tensor_scale": (_int, [_vp, _vp, _i64, _i64, _i64, _f32, _vp, _vp, _vp]),
     "wush_quant_int8": (_int, [_vp, _int, _i64, _i64, _vp, _vp, _vp]),
-    "wush_w8a8_gemm": (_int, [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp, _int, _vp]),
+    "wush_w8a8_gemm_workspace_bytes": (_sz, [_i64, _i64]),
+    "wush_w8a8_gemm": (_int, [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp, _int, _vp, _sz, _vp]),
     "wush_w8a8_linear_workspace_bytes": (_sz, [_i64, _i64]),
     "wush_w8a8_linear": (_int, [_vp, _int, _vp, _vp, _vp, _i64, _i64, _i64, _vp, _vp, _sz, _vp]),
     "wush_expert_sort": (_int, [_vp, _int, _i64, _i64, _i64, _vp, _vp, _vp]),
@@ -49,8 +50,8 @@ SIGNATURES = {
     "wush_expert_gather_quant_int8": (_int, [_vp, _int, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _vp]),
     "wush_expert_combine": (_int, [_vp, _int, _i64, _i64, _vp, _i64, _vp, _vp, _vp]),
     "wush_expert_combine_grad": (_int, [_vp, _vp, _int, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp]),
-    "wush_w8a8_grouped_gemm": (_int, [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _int, _vp]),
-    "wush_w8a8_grouped_gated": (_int, [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _vp]),
+    "wush_w8a8_grouped_gemm": (_int, [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _int, _vp, _sz, _vp]),
+    "wush_w8a8_grouped_gated": (_int, [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _vp, _sz, _vp]),
     "wush_w8a8_expert_ffn_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64, _i64]),
     "wush_w8a8_expert_ffn": (_int, [_vp, _int, _vp, _int, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _vp, _vp,
                                     _sz, _vp]),

@@ -335,6 +335,14 @@ const float* check_bias(const c10::optional<torch::Tensor>& bias, const torch::T
     return bias->data_ptr<float>();
 }
 
+// Scratch of a product of 8-bit codes; undefined where none is needed.
+torch::Tensor product_scratch(int64_t rows, int64_t experts, const torch::Tensor& like, size_t* nbytes)
+{
+    *nbytes = wush_w8a8_gemm_workspace_bytes(rows, experts);
+    return *nbytes ? torch::empty({(int64_t)*nbytes}, like.options().dtype(torch::kUInt8)) : torch::Tensor();
+}
+void* ptr_or_null(const torch::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+
 int out_code(torch::ScalarType d, const char* op)
 {
     TORCH_CHECK(d == torch::kHalf || d == torch::kBFloat16, op, ": out_dtype must be torch.float16 or torch.bfloat16");
@@ -353,8 +361,11 @@ torch::Tensor w8a8_gemm(torch::Tensor xq, torch::Tensor xs, torch::Tensor wq, to
     const int code = out_code(out_dtype, op);
     const at::cuda::OptionalCUDAGuard guard(xq.device());
     auto y = torch::empty(with_last(xq, N), xq.options().dtype(out_dtype));
+    size_t nbytes;
+    auto work = product_scratch(xq.numel() / K, 1, xq, &nbytes);
     check_status(wush_w8a8_gemm(xq.data_ptr<int8_t>(), xs.data_ptr<float>(), wq.data_ptr<int8_t>(), ws.data_ptr<float>(),
-                                check_bias(bias, xq, N, op), xq.numel() / K, N, K, y.data_ptr(), code, stream_of(xq)),
+                                check_bias(bias, xq, N, op), xq.numel() / K, N, K, y.data_ptr(), code, ptr_or_null(work), nbytes,
+                                stream_of(xq)),
                  op);
     return y;
 }
@@ -521,8 +532,11 @@ torch::Tensor w8a8_grouped_gemm(torch::Tensor xq, torch::Tensor xs, torch::Tenso
     const int code = out_code(out_dtype, op);
     const at::cuda::OptionalCUDAGuard guard(xq.device());
     auto y = torch::empty({g.rows, g.N}, xq.options().dtype(out_dtype));
+    size_t nbytes;
+    auto work = product_scratch(g.rows, g.experts, xq, &nbytes);
     check_status(wush_w8a8_grouped_gemm(xq.data_ptr<int8_t>(), xs.data_ptr<float>(), wq.data_ptr<int8_t>(), ws.data_ptr<float>(),
-                                        offsets.data_ptr<int32_t>(), g.rows, g.experts, g.N, g.K, y.data_ptr(), code, stream_of(xq)),
+                                        offsets.data_ptr<int32_t>(), g.rows, g.experts, g.N, g.K, y.data_ptr(), code,
+                                        ptr_or_null(work), nbytes, stream_of(xq)),
                  op);
     return y;
 }
@@ -534,9 +548,11 @@ torch::Tensor w8a8_grouped_gated(torch::Tensor xq, torch::Tensor xs, torch::Tens
     TORCH_CHECK(g.N % 2 == 0, op, ": wq must be (experts, 2 * I, K), the gate channels first");
     const at::cuda::OptionalCUDAGuard guard(xq.device());
     auto h = torch::empty({g.rows, g.N / 2}, xq.options().dtype(torch::kFloat32));
+    size_t nbytes;
+    auto work = product_scratch(g.rows, g.experts, xq, &nbytes);
     check_status(wush_w8a8_grouped_gated(xq.data_ptr<int8_t>(), xs.data_ptr<float>(), wq.data_ptr<int8_t>(), ws.data_ptr<float>(),
                                          offsets.data_ptr<int32_t>(), g.rows, g.experts, g.N / 2, g.K, h.data_ptr<float>(),
-                                         stream_of(xq)),
+                                         ptr_or_null(work), nbytes, stream_of(xq)),
                  op);
     return h;
 }

@@ -14,9 +14,8 @@
 // rows of the same channels, INTERLEAVED in shared memory by the order of the dimensions, so gate and up of a channel end
 // in neighbouring lanes of tensor memory and meet in one shuffle.  Rows beyond the channels of an expert read as zero.
 //
-// One tile per cluster of S CTAs, each with 1/S of K; the partial sums meet in distributed shared memory, every CTA
-// finishing the columns of 1/S of the tokens.  Splitting K is what keeps all multiprocessors streaming when a layer has few
-// tiles, and shortens the last, partly filled wave when it has many.
+// Up to 64 tokens per expert: persistent CTAs, one per multiprocessor, that stream weights without a pause (below).
+// More: CTA pairs on 256 x 256 tiles (further down).
 //
 // Roles per CTA (192 threads): warp 0 TMA producer, warp 1 MMA issuer (and owner of the tensor memory), warps 2-5 epilogue.
 // Every wait is bounded; one that gives up leaves a role code in a device word (wush_device_flag, bits 16-23).
@@ -34,17 +33,16 @@ __device__ int g_w8a8_err;
 
 constexpr int THREADS = 192;
 constexpr int A_BYTES = 128 * 128;                       // 128 weight rows of 128 bytes per stage
-constexpr int MAX_SPLIT = 8;
 
-// Shared memory: stages, then the exchange buffer (NT x 128 sums), then token scales and barriers.
-template <int NT> struct Small {
+// Shared memory of the streaming kernel: stages, token scales of two tiles, the table of tiles, barriers.
+template <int NT> struct Stream {
     static constexpr int STAGE = A_BYTES + NT * 128;
-    // two CTAs per multiprocessor: 113 KB each
-    static constexpr int EXCHANGE = NT * 512;
-    static constexpr int FIXED = EXCHANGE + NT * 4 + 256 + 1024;
-    static constexpr int STAGES = (113 * 1024 - FIXED) / STAGE;
+    static constexpr int TABLE_BYTES = 2 * (WUSH_EXPERT_MAX + 2) * 4;
+    static constexpr int FIXED = 2 * NT * 4 + TABLE_BYTES + 256 + 1024;
+    static constexpr int STAGES = (226 * 1024 - FIXED) / STAGE;
     static constexpr int SMEM = STAGES * STAGE + FIXED;
-    static constexpr int COLS = NT < 32 ? 32 : NT;       // columns of tensor memory
+    static constexpr int COLS = 2 * NT < 32 ? 32 : 2 * NT;           // columns of tensor memory: two accumulators
+    static constexpr int PIECE = 128 * NT;                           // sums of a tile
 };
 
 struct Params {
@@ -57,6 +55,8 @@ struct Params {
     int K, experts, tiles_c;     // tiles_c: channel tiles
     int bf16_out;
     int early;                   // weights (and offsets) may be read before the kernel in front has finished
+    int32_t* counters;           // one per CTA, zero; null: no tile is split
+    uint32_t* pieces;            // two per CTA
 };
 
 __device__ __forceinline__ uint64_t desc_sw128(uint32_t saddr)
@@ -88,57 +88,11 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* r)
         : "r"(taddr)
         : "memory");
 }
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
-__device__ __forceinline__ uint32_t cluster_size() { uint32_t r; asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(r)); return r; }
-__device__ __forceinline__ void st_cluster(uint32_t addr, uint32_t v)
-{
-    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
-}
-
 // First row of expert e.  Offsets come from the caller: kept inside the rows, so that a bad one reads nothing out of range.
 __device__ __forceinline__ int64_t first_row(const Params& p, int e)
 {
     const int32_t v = __ldcg(p.offsets + e);
     return v < 0 ? 0 : (v < p.rows ? (int64_t)v : p.rows);
-}
-
-// Expert, first row and row count of token tile `slot` (tiles of NT rows, counted expert by expert).  One full warp; false
-// if there are fewer tiles.
-__device__ __forceinline__ bool find_tile(const Params& p, int slot, int nt, int& expert, int64_t& row0, int& n_rows)
-{
-    if (!p.offsets) {
-        expert = 0;
-        row0 = (int64_t)slot * nt;
-        if (row0 >= p.rows) return false;
-        n_rows = (int)min((int64_t)nt, p.rows - row0);
-        return true;
-    }
-    const int lane = threadIdx.x & 31;
-    int before = 0;
-    for (int e0 = 0; e0 < p.experts; e0 += 32) {
-        const int e = e0 + lane;
-        int64_t a = 0, b = 0;
-        if (e < p.experts) { a = first_row(p, e); b = first_row(p, e + 1); }
-        const int tiles = b > a ? (int)((b - a + nt - 1) / nt) : 0;
-        int scan = tiles;
-#pragma unroll
-        for (int d = 1; d < 32; d *= 2) {
-            const int up = __shfl_up_sync(0xffffffffu, scan, d);
-            if (lane >= d) scan += up;
-        }
-        const uint32_t hit = __ballot_sync(0xffffffffu, before + scan > slot);
-        if (hit) {
-            const int src = __ffs(hit) - 1;
-            const int64_t start = a + (int64_t)(slot - (before + scan - tiles)) * nt;
-            row0 = __shfl_sync(0xffffffffu, start, src);
-            n_rows = (int)min((int64_t)nt, __shfl_sync(0xffffffffu, b, src) - row0);
-            expert = e0 + src;
-            return true;
-        }
-        before += __shfl_sync(0xffffffffu, scan, 31);
-    }
-    return false;
 }
 
 // What a thread of the epilogue needs to turn the sums of its channel into results.
@@ -150,93 +104,200 @@ struct Lane {
     const float* sx;             // token scales in shared memory
 };
 
-// Results of two neighbouring tokens m, m + 1 (m even within the tile).  The two lanes of a pair exchange one value each:
-// the even lane ends with both values of token m, the odd lane with both of token m + 1, so that 16-bit results leave as
-// 4-byte stores (64 bytes per token and warp) and a gated pair meets without another exchange.
-template <bool GATED>
-__device__ __forceinline__ void emit_pair(const Params& p, const Lane& L, int m, uint32_t a0, uint32_t a1)
+// Results of COUNT tokens from m0 (even) on.  The two lanes of a pair exchange one value for every two tokens m, m + 1: the
+// even lane ends with both values of token m, the odd lane with both of token m + 1, so that 16-bit results leave as 4-byte
+// stores (64 bytes per token and warp) and a gated pair meets without another exchange.  Straight-line code: a branch per
+// pair left the warp waiting for one shuffle after another (14 us per 128 x 256 tile, 4 with this).
+template <bool GATED, int COUNT>
+__device__ __forceinline__ void emit(const Params& p, const Lane& L, int m0, const uint32_t* v)
 {
-    const float2 sx = *reinterpret_cast<const float2*>(L.sx + m);
-    float f0 = __fmul_rn((float)(int)a0, __fmul_rn(sx.x, L.sw));
-    float f1 = __fmul_rn((float)(int)a1, __fmul_rn(sx.y, L.sw));
-    const bool odd = threadIdx.x & 1;
+    const int odd = threadIdx.x & 1;
+    const int left = L.n_rows - m0;                      // tokens that exist
+    if (left <= 0) return;
+    auto scaled = [&](int j) { return __fmul_rn((float)(int)v[j], __fmul_rn(L.sx[m0 + j], L.sw)); };
     if constexpr (GATED) {
-        const float got = __shfl_xor_sync(0xffffffffu, odd ? f0 : f1, 1);
-        const float g = odd ? got : f0, u = odd ? f1 : got;
-        const int t = m + odd;
-        if (t < L.n_rows && L.n < p.N)
-            reinterpret_cast<float*>(p.y)[(L.row0 + t) * p.N + L.n] = __fmul_rn(__fdividef(g, 1.f + expf(-g)), u);
-    } else {
-        f0 = __fadd_rn(f0, L.bias);
-        f1 = __fadd_rn(f1, L.bias);
-        if ((p.N & 1) == 0) {
+        float* y = reinterpret_cast<float*>(p.y) + (L.row0 + m0 + odd) * p.N + L.n;
+        const bool mine = L.n < p.N;
+#pragma unroll
+        for (int j = 0; j < COUNT; j += 2) {
+            const float f0 = scaled(j), f1 = scaled(j + 1);
+            const float got = __shfl_xor_sync(0xffffffffu, odd ? f0 : f1, 1);
+            const float g = odd ? got : f0, u = odd ? f1 : got;
+            const float h = __fmul_rn(__fdividef(g, 1.f + expf(-g)), u);
+            if (mine && j + odd < left) *y = h;
+            y += 2 * p.N;
+        }
+    } else if ((p.N & 1) == 0) {
+        const int64_t n = L.n & ~int64_t(1);
+        uint32_t* y = reinterpret_cast<uint32_t*>(reinterpret_cast<uint16_t*>(p.y) + (L.row0 + m0 + odd) * p.N + n);
+        const bool mine = n < p.N;
+#pragma unroll
+        for (int j = 0; j < COUNT; j += 2) {
+            const float f0 = __fadd_rn(scaled(j), L.bias), f1 = __fadd_rn(scaled(j + 1), L.bias);
             const float got = __shfl_xor_sync(0xffffffffu, odd ? f0 : f1, 1);
             const float lo = odd ? got : f0, hi = odd ? f1 : got;
-            const int t = m + odd;
-            const int64_t n = L.n & ~int64_t(1);
-            if (t < L.n_rows && n < p.N) {
-                uint32_t w;
-                if (p.bf16_out) { __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi); w = *reinterpret_cast<uint32_t*>(&h); }
-                else { __half2 h = __floats2half2_rn(lo, hi); w = *reinterpret_cast<uint32_t*>(&h); }
-                *reinterpret_cast<uint32_t*>(reinterpret_cast<uint16_t*>(p.y) + (L.row0 + t) * p.N + n) = w;
-            }
-        } else if (L.n < p.N) {
-            uint16_t* y = reinterpret_cast<uint16_t*>(p.y) + (L.row0 + m) * p.N + L.n;
+            uint32_t w;
+            if (p.bf16_out) { __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi); w = *reinterpret_cast<uint32_t*>(&h); }
+            else { __half2 h = __floats2half2_rn(lo, hi); w = *reinterpret_cast<uint32_t*>(&h); }
+            if (mine && j + odd < left) *y = w;
+            y += p.N;
+        }
+    } else {                                             // rows of an odd number of channels: 2-byte stores
+        uint16_t* y = reinterpret_cast<uint16_t*>(p.y) + (L.row0 + m0) * p.N + L.n;
+        const bool mine = L.n < p.N;
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
-                if (m + i < L.n_rows) {
-                    const float f = i ? f1 : f0;
-                    y[i * p.N] = p.bf16_out ? __bfloat16_as_ushort(__float2bfloat16_rn(f)) : __half_as_ushort(__float2half_rn(f));
-                }
+        for (int j = 0; j < COUNT; ++j) {
+            const float f = __fadd_rn(scaled(j), L.bias);
+            const uint16_t w = p.bf16_out ? __bfloat16_as_ushort(__float2bfloat16_rn(f)) : __half_as_ushort(__float2half_rn(f));
+            if (mine && j < left) *y = w;
+            y += p.N;
         }
     }
 }
 
-// Rows behind the last expert's are zero: written by the CTAs that own column tile `ct`, rows dealt over `parts`.
+struct Tile {
+    int expert, ct, n_rows, nt;  // nt: token columns of the tile
+    int64_t row0;
+};
+
+// Scale and bias of this lane's channel `c` (0..127) of the tile; `first`: first result channel of the CTA's 128 weight rows.
 template <bool GATED>
-__device__ __forceinline__ void zero_tail(const Params& p, int ct, int part, int parts, int tid, int threads)
+__device__ __forceinline__ Lane make_lane(const Params& p, const Tile& t, int64_t first, int c, const float* sx)
 {
-    constexpr int WIDTH = GATED ? 64 : 128;
-    const int64_t n0 = (int64_t)ct * WIDTH;
-    for (int64_t r = first_row(p, p.experts) + part; r < p.rows; r += parts)
-        for (int i = tid; i < WIDTH && n0 + i < p.N; i += threads) {
-            if constexpr (GATED) reinterpret_cast<float*>(p.y)[r * p.N + n0 + i] = 0.f;
-            else reinterpret_cast<uint16_t*>(p.y)[r * p.N + n0 + i] = 0;
+    Lane L;
+    L.row0 = t.row0;
+    L.n_rows = t.n_rows;
+    L.n = first + (GATED ? c >> 1 : c);
+    L.sw = 0.f;
+    L.bias = 0.f;
+    L.sx = sx;
+    if (L.n < p.N) {
+        L.sw = p.ws[(int64_t)t.expert * (GATED ? 2 * p.N : p.N) + L.n + (GATED && (c & 1) ? p.N : 0)];
+        if (!GATED && p.bias) L.bias = p.bias[L.n];
+    }
+    return L;
+}
+
+// The table of tiles of a grouped product, by one warp: first[e] = first tile of expert e, row[e] = its first row.
+template <typename Tiles>
+__device__ __forceinline__ void make_table(const Params& p, int32_t* first, int32_t* row, Tiles tiles_of)
+{
+    const int lane = threadIdx.x & 31;
+    int before = 0;
+    for (int e0 = 0; e0 < p.experts; e0 += 32) {
+        const int e = e0 + lane;
+        int64_t a = 0, b = 0;
+        if (e < p.experts) { a = first_row(p, e); b = first_row(p, e + 1); }
+        const int tiles = b > a ? tiles_of(b - a) * p.tiles_c : 0;
+        int scan = tiles;
+#pragma unroll
+        for (int d = 1; d < 32; d *= 2) {
+            const int up = __shfl_up_sync(0xffffffffu, scan, d);
+            if (lane >= d) scan += up;
+        }
+        if (e < p.experts) {
+            first[e] = before + scan - tiles;
+            row[e] = (int32_t)a;
+            if (e == p.experts - 1) { first[e + 1] = before + scan; row[e + 1] = (int32_t)b; }
+        }
+        before += __shfl_sync(0xffffffffu, scan, 31);
+    }
+}
+
+// Rows behind the last expert's become zero: dealt to the CTAs, written by the epilogue's 128 threads.
+template <bool GATED>
+__device__ __forceinline__ void zero_tail(const Params& p, int64_t used, int tid)
+{
+    for (int64_t r = used + blockIdx.x; r < p.rows; r += gridDim.x)
+        for (int64_t i = tid; i < p.N; i += 128) {
+            if constexpr (GATED) reinterpret_cast<float*>(p.y)[r * p.N + i] = 0.f;
+            else reinterpret_cast<uint16_t*>(p.y)[r * p.N + i] = 0;
         }
 }
+
+// ---- few tokens: weights streamed by persistent CTAs -----------------------------------------------------------------------
+// Bound by the bytes of the weights.  One CTA per multiprocessor with a ring of 8 to 12 stages (128 weight rows x 128 bytes
+// each, 190 KB and more in flight), a producer that runs ahead over tile borders and two accumulators, so that the stream
+// does not pause for a tile's end.  Work is the sequence of all stages, tile after tile, cut into one contiguous run per CTA.
+// Runs end at tile borders where that costs no more than FIXUP_STAGES stages of balance; otherwise they are of equal length,
+// and a tile cut by a border is finished by whichever of its CTAs comes last: every CTA leaves its sums in a slot of the
+// workspace and counts itself in, and the last one adds the slots (int32: in any order the same sum).  Nobody waits.
+constexpr int FIXUP_STAGES = 8;
+
+struct Run {
+    int64_t begin, end;          // stages of this CTA
+    int64_t total;
+    int ctas;                    // CTAs that have a run
+    bool split;
+};
+__device__ __forceinline__ Run make_run(const Params& p, int64_t tiles, int k_steps, int cta, int ctas)
+{
+    Run r;
+    r.total = tiles * k_steps;
+    const int64_t whole = (tiles + ctas - 1) / ctas * k_steps, even = (r.total + ctas - 1) / ctas + FIXUP_STAGES;
+    r.split = p.counters && whole > even;
+    r.ctas = r.split ? (int)min((int64_t)ctas, r.total) : ctas;
+    if (cta >= r.ctas) r.begin = r.end = 0;
+    else if (r.split) { r.begin = r.total * cta / r.ctas; r.end = r.total * (cta + 1) / r.ctas; }
+    else { r.begin = tiles * cta / ctas * k_steps; r.end = tiles * (cta + 1) / ctas * k_steps; }
+    return r;
+}
+// The CTA of a split whose run holds `stage`: the last one that begins at or before it.
+__device__ __forceinline__ int owner(const Run& r, int64_t stage) { return (int)(((stage + 1) * r.ctas - 1) / r.total); }
+
+template <int NT>
+struct StreamOrder {
+    const Params& p;
+    const int32_t* first;
+    const int32_t* row;
+    int e;
+
+    __device__ __forceinline__ Tile at(int t)
+    {
+        Tile r;
+        int64_t start = 0, count = p.rows;
+        int local = t;
+        if (first) {
+            while (t >= first[e + 1]) ++e;
+            start = row[e];
+            count = row[e + 1] - row[e];
+            local = t - first[e];
+        }
+        const int tiles = (int)((count + NT - 1) / NT), tok = local % tiles;     // tokens fastest: the weights come from L2 then
+        r.ct = local / tiles;
+        r.nt = NT;
+        r.expert = e;
+        r.row0 = start + (int64_t)tok * NT;
+        r.n_rows = (int)min((int64_t)NT, count - (int64_t)tok * NT);
+        return r;
+    }
+};
 
 template <int NT, bool GATED>
-__global__ void __launch_bounds__(THREADS, 2) w8a8_small_kernel(const __grid_constant__ CUtensorMap map_w,
-                                                                const __grid_constant__ CUtensorMap map_x, const Params p)
+__global__ void __launch_bounds__(THREADS, 1) w8a8_stream_kernel(const __grid_constant__ CUtensorMap map_w,
+                                                                 const __grid_constant__ CUtensorMap map_x, const Params p)
 {
-    using C = Small<NT>;
+    using C = Stream<NT>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint32_t* exchange = reinterpret_cast<uint32_t*>(smem + C::STAGES * C::STAGE);
-    float* sx_s = reinterpret_cast<float*>(smem + C::STAGES * C::STAGE + C::EXCHANGE);
-    uint64_t* full = reinterpret_cast<uint64_t*>(sx_s + NT);
+    float* sx_s = reinterpret_cast<float*>(smem + C::STAGES * C::STAGE);
+    int32_t* first_s = reinterpret_cast<int32_t*>(sx_s + 2 * NT);
+    int32_t* row_s = first_s + WUSH_EXPERT_MAX + 2;
+    uint64_t* full = reinterpret_cast<uint64_t*>(row_s + WUSH_EXPERT_MAX + 2);
     uint64_t* empty = full + C::STAGES;
-    uint64_t* done = empty + C::STAGES;
+    uint64_t* acc_full = empty + C::STAGES;
+    uint64_t* acc_empty = acc_full + 2;
+    uint64_t* done = acc_empty + 2;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+    int* last_s = reinterpret_cast<int*>(tmem_slot + 1);                 // [2]
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const uint32_t split = cluster_size(), rank = split > 1 ? tc::cluster_ctarank() : 0;
-    const int tile = blockIdx.x / split, slot = tile / p.tiles_c, ct = tile - slot * p.tiles_c;
-    const int n_slots = gridDim.x / split / p.tiles_c;
-
     if (!p.early) pdl_wait();
-    int expert, n_rows;
-    int64_t row0;
-    const bool any = find_tile(p, slot, NT, expert, row0, n_rows);       // the same in every warp and CTA of the cluster
-    if (!any) {
-        if (p.early) pdl_wait();
-        pdl_launch_dependents();
-        if (rank == 0 && p.offsets) zero_tail<GATED>(p, ct, slot, n_slots, tid, THREADS);
-        return;
-    }
-
     if (tid == 0) {
+        tc::prefetch_tensormap(&map_w);
+        tc::prefetch_tensormap(&map_x);
         for (int i = 0; i < C::STAGES; ++i) { tc::mbar_init(&full[i], 1); tc::mbar_init(&empty[i], 1); }
+        for (int i = 0; i < 2; ++i) { tc::mbar_init(&acc_full[i], 1); tc::mbar_init(&acc_empty[i], 4); }
         tc::mbar_init(done, 1);
         tc::mbar_fence_init();
     }
@@ -244,35 +305,53 @@ __global__ void __launch_bounds__(THREADS, 2) w8a8_small_kernel(const __grid_con
         tc::tmem_alloc(tmem_slot, C::COLS);
         tc::tmem_relinquish();
     }
+    if (warp == 2 && p.offsets) make_table(p, first_s, row_s, [](int64_t n) { return (int)((n + NT - 1) / NT); });
     tc::tc_fence_before();
     __syncthreads();
     tc::tc_fence_after();
-    if (split > 1) cluster_arrive();                                     // waited for before anything goes to another CTA
     const uint32_t tmem = *tmem_slot;
-    const int all_steps = (p.K + 127) / 128;
-    const int k_first = (int)((int64_t)all_steps * rank / split), k_steps = (int)((int64_t)all_steps * (rank + 1) / split) - k_first;
-    bool ok = true;
+    const int k_steps = (p.K + 127) / 128;
+    const int n_tiles = p.offsets ? first_s[p.experts] : (int)((p.rows + NT - 1) / NT) * p.tiles_c;
+    const Run run = make_run(p, n_tiles, k_steps, blockIdx.x, gridDim.x);
+    StreamOrder<NT> order = {p, p.offsets ? first_s : nullptr, row_s, 0};
+    constexpr int WIDTH = GATED ? 64 : 128;
 
     if (warp == 0) {
         if (lane == 0) {
-            const int c_w = ct * (GATED ? 64 : 128);
-            const int ahead = k_steps < C::STAGES ? k_steps : C::STAGES;
+            const int n = (int)(run.end - run.begin);
+            int t = n ? (int)(run.begin / k_steps) : 0, ks = n ? (int)(run.begin - (int64_t)t * k_steps) : 0;
+            Tile tile = {};
+            if (n) tile = order.at(t);
+            const int t_first = t, ks_first = ks;
+            auto step = [&](bool more) {
+                if (++ks == k_steps) { ks = 0; ++t; if (more) tile = order.at(t); }
+            };
+            const int ahead = n < C::STAGES ? n : C::STAGES;
             for (int i = 0; i < ahead; ++i) {                            // the weights do not depend on the kernel in front
                 tc::mbar_expect_tx(&full[i], C::STAGE);
-                tma_load_4d(smem + i * C::STAGE, &map_w, &full[i], (k_first + i) * 128, 0, c_w, expert);
+                tma_load_4d(smem + i * C::STAGE, &map_w, &full[i], ks * 128, 0, tile.ct * WIDTH, tile.expert);
+                step(i + 1 < n);
             }
+            const int t_next = t, ks_next = ks;
             if (p.early) pdl_wait();
-            for (int i = 0; i < ahead; ++i)
-                tc::tma_load_2d(smem + i * C::STAGE + A_BYTES, &map_x, &full[i], (k_first + i) * 128, (int)row0);
+            if (n) { order.e = 0; t = t_first; ks = ks_first; tile = order.at(t); }
+            for (int i = 0; i < ahead; ++i) {
+                tc::tma_load_2d(smem + i * C::STAGE + A_BYTES, &map_x, &full[i], ks * 128, (int)tile.row0);
+                step(i + 1 < n);
+            }
+            t = t_next;
+            ks = ks_next;
             int issued = ahead;
             uint32_t s = 0, phase = 0;
-            for (int ks = ahead; ks < k_steps; ++ks) {
+            bool ok = true;
+            for (int i = ahead; i < n; ++i) {
                 if (!tc::mbar_wait(&empty[s], phase)) { ok = false; break; }
                 tc::mbar_expect_tx(&full[s], C::STAGE);
-                tma_load_4d(smem + s * C::STAGE, &map_w, &full[s], (k_first + ks) * 128, 0, c_w, expert);
-                tc::tma_load_2d(smem + s * C::STAGE + A_BYTES, &map_x, &full[s], (k_first + ks) * 128, (int)row0);
+                tma_load_4d(smem + s * C::STAGE, &map_w, &full[s], ks * 128, 0, tile.ct * WIDTH, tile.expert);
+                tc::tma_load_2d(smem + s * C::STAGE + A_BYTES, &map_x, &full[s], ks * 128, (int)tile.row0);
                 ++issued;
                 if (++s == C::STAGES) { s = 0; phase ^= 1; }
+                step(i + 1 < n);
             }
             if (!ok) {                                                   // copies in flight land before the memory is given back
                 atomicExch(&g_w8a8_err, 1);
@@ -283,88 +362,98 @@ __global__ void __launch_bounds__(THREADS, 2) w8a8_small_kernel(const __grid_con
         }
     } else if (warp == 1) {
         if (lane == 0) {
-            uint32_t s = 0, phase = 0;
+            uint32_t s = 0, phase = 0, ab = 0, aphase = 0;
             const uint32_t idesc = tc::idesc_i8(NT);
-            for (int ks = 0; ks < k_steps; ++ks) {
-                if (!tc::mbar_wait(&full[s], phase)) { ok = false; break; }
+            bool ok = true;
+            for (int64_t at = run.begin; at < run.end && ok;) {
+                const int k0 = (int)(at % k_steps), k1 = (int)min((int64_t)k_steps, k0 + run.end - at);
+                if (!tc::mbar_wait(&acc_empty[ab], aphase ^ 1)) { ok = false; break; }
                 tc::tc_fence_after();
-                const uint32_t sa = tc::smem_u32(smem + s * C::STAGE), sb = sa + A_BYTES;
+                for (int ks = k0; ks < k1; ++ks) {
+                    if (!tc::mbar_wait(&full[s], phase)) { ok = false; break; }
+                    tc::tc_fence_after();
+                    const uint32_t sa = tc::smem_u32(smem + s * C::STAGE), sb = sa + A_BYTES;
 #pragma unroll
-                for (int kk = 0; kk < 4; ++kk)
-                    tc::mma_i8(tmem, desc_sw128(sa + kk * 32), desc_sw128(sb + kk * 32), idesc, (ks | kk) ? 1u : 0u);
-                tc::mma_commit(&empty[s]);
-                if (++s == C::STAGES) { s = 0; phase ^= 1; }
+                    for (int kk = 0; kk < 4; ++kk)
+                        tc::mma_i8(tmem + ab * NT, desc_sw128(sa + kk * 32), desc_sw128(sb + kk * 32), idesc, (ks - k0) | kk ? 1u : 0u);
+                    tc::mma_commit(&empty[s]);
+                    if (++s == C::STAGES) { s = 0; phase ^= 1; }
+                }
+                if (!ok) break;
+                tc::mma_commit(&acc_full[ab]);
+                if (++ab == 2) { ab = 0; aphase ^= 1; }
+                at += k1 - k0;
             }
             if (!ok) atomicExch(&g_w8a8_err, 2);
             tc::mma_commit(done);
             for (uint32_t spin = 0; spin < WUSH_SPIN_LIMIT; ++spin)
                 if (tc::mbar_try_wait(done, 0)) break;
         }
-    }
-
-    const int quarter = warp & 3, c = quarter * 32 + lane;               // tcgen05.ld: a warp reads lanes 32 * (warp % 4) ...
-    Lane L;
-    if (warp >= 2) {
+    } else {
         if (p.early) pdl_wait();
         pdl_launch_dependents();
-        L.row0 = row0;
-        L.n_rows = n_rows;
-        L.n = GATED ? (int64_t)ct * 64 + (c >> 1) : (int64_t)ct * 128 + c;
-        L.sx = sx_s;
-        L.sw = 0.f;
-        L.bias = 0.f;
-        if (L.n < p.N) {
-            L.sw = p.ws[(int64_t)expert * (GATED ? 2 * p.N : p.N) + L.n + (GATED && (c & 1) ? p.N : 0)];
-            if (!GATED && p.bias) L.bias = p.bias[L.n];
+        const int quarter = warp & 3, c = quarter * 32 + lane;           // tcgen05.ld: a warp reads lanes 32 * (warp % 4) ...
+        if (p.offsets) zero_tail<GATED>(p, row_s[p.experts], tid - 64);
+        uint32_t ab = 0, aphase = 0;
+        bool ok = true;                                                  // after a give-up: no more work, but every barrier of the warps
+        for (int64_t at = run.begin; at < run.end;) {
+            const int t = (int)(at / k_steps), k0 = (int)(at - (int64_t)t * k_steps), k1 = (int)min((int64_t)k_steps, k0 + run.end - at);
+            const Tile tile = order.at(t);
+            float* sx = sx_s + ab * NT;
+            const Lane L = make_lane<GATED>(p, tile, (int64_t)tile.ct * WIDTH, c, sx);
+            for (int i = tid - 64; i < NT; i += THREADS - 64) sx[i] = i < tile.n_rows ? p.xs[tile.row0 + i] : 0.f;
+            asm volatile("bar.sync 1, 128;" ::: "memory");               // the epilogue's own barrier
+            if (ok) ok = __all_sync(0xffffffffu, tc::mbar_wait(&acc_full[ab], aphase));
+            tc::tc_fence_after();
+            const uint32_t base = tmem + ((uint32_t)(quarter * 32) << 16) + ab * NT;
+            const bool whole = k1 - k0 == k_steps;
+            uint32_t* slot = whole ? nullptr : p.pieces + (size_t)(2 * blockIdx.x + (k0 == 0)) * C::PIECE + c;
+#pragma unroll
+            for (int c0 = 0; c0 < NT; c0 += 16) {
+                uint32_t v[16];
+                tmem_ld16(base + c0, v);
+                tc::tmem_ld_wait();
+                if (c0 == NT - 16) {
+                    tc::tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) tc::mbar_arrive(&acc_empty[ab]);
+                }
+                if (whole) {
+                    if (ok) emit<GATED, 16>(p, L, c0, v);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) __stcg(slot + (c0 + j) * 128, v[j]);
+                }
+            }
+            if (!whole) {
+                const int c_first = owner(run, (int64_t)t * k_steps), c_last = owner(run, (int64_t)t * k_steps + k_steps - 1);
+                __threadfence();
+                asm volatile("bar.sync 1, 128;" ::: "memory");
+                if (tid == 64) {
+                    last_s[ab] = atomicAdd(p.counters + c_first, 1) == c_last - c_first;
+                    __threadfence();
+                }
+                asm volatile("bar.sync 1, 128;" ::: "memory");
+                if (last_s[ab] && ok) {
+                    __threadfence();
+#pragma unroll 1
+                    for (int c0 = 0; c0 < NT && c0 < tile.n_rows; c0 += 16) {
+                        uint32_t v[16];
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) v[j] = 0;
+                        for (int k = c_first; k <= c_last; ++k) {
+                            const uint32_t* from = p.pieces + (size_t)(2 * k + (k == c_first)) * C::PIECE + c0 * 128 + c;
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) v[j] += __ldcg(from + j * 128);
+                        }
+                        emit<GATED, 16>(p, L, c0, v);
+                    }
+                }
+            }
+            if (++ab == 2) { ab = 0; aphase ^= 1; }
+            at += k1 - k0;
         }
-        for (int i = tid - 64; i < NT; i += THREADS - 64) sx_s[i] = i < n_rows ? p.xs[row0 + i] : 0.f;
-        asm volatile("bar.sync 1, 128;" ::: "memory");                   // the epilogue's own barrier
-        if (rank == 0 && p.offsets) zero_tail<GATED>(p, ct, slot, n_slots, tid - 64, THREADS - 64);
-        ok = tc::mbar_wait(done, 0);
         if (!ok && lane == 0) atomicExch(&g_w8a8_err, 4);
-        tc::tc_fence_after();
-    }
-    __syncwarp();
-    if (split > 1) cluster_wait();                                       // every CTA of the cluster has started
-    if (warp >= 2) {
-        const uint32_t base = tmem + ((uint32_t)(quarter * 32) << 16);
-        const uint32_t slice = NT / split, shift = 31 - __clz(slice);
-#pragma unroll
-        for (int c0 = 0; c0 < NT; c0 += 16) {
-            uint32_t v[16];
-            tmem_ld16(base + c0, v);
-            tc::tmem_ld_wait();
-            if (split == 1) {
-                if (ok) {
-#pragma unroll
-                    for (int j = 0; j < 16; j += 2)
-                        if (c0 + j < n_rows) emit_pair<GATED>(p, L, c0 + j, v[j], v[j + 1]);
-                }
-            } else {
-#pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    const uint32_t col = c0 + j;
-                    st_cluster(tc::map_to_rank(exchange + (rank * slice + (col & (slice - 1))) * 128 + c, col >> shift), v[j]);
-                }
-            }
-        }
-    }
-    if (split > 1) {
-        __syncwarp();
-        cluster_arrive();
-        cluster_wait();
-        if (warp >= 2 && ok) {
-            const int slice = NT / split, m0 = (int)rank * slice;
-            for (int m = 0; m < slice; m += 2) {
-                if (m0 + m >= n_rows) break;
-                uint32_t a0 = 0, a1 = 0;
-                for (uint32_t r = 0; r < split; ++r) {
-                    a0 += exchange[(r * slice + m) * 128 + c];
-                    a1 += exchange[(r * slice + m + 1) * 128 + c];
-                }
-                emit_pair<GATED>(p, L, m0 + m, a0, a1);
-            }
-        }
     }
     tc::tc_fence_before();
     __syncthreads();
@@ -398,11 +487,6 @@ __device__ __forceinline__ void tma_load_4d_pair(void* dst, const CUtensorMap* m
         "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
         : "memory");
 }
-
-struct Tile {
-    int expert, ct, n_rows, nt;  // nt: token columns of the tile, a multiple of 32
-    int64_t row0;
-};
 
 // Token tiles of `count` rows: as few as possible, of equal size.  (tiles - 1) * nt < count, because nt <= 256.
 __host__ __device__ __forceinline__ int token_tiles(int64_t count) { return (int)((count + PAIR_TOKENS - 1) / PAIR_TOKENS); }
@@ -478,27 +562,7 @@ w8a8_pair_kernel(const __grid_constant__ PairMaps maps, const Params p, int band
         tc::tmem_alloc_pair(tmem_slot, 512);
         tc::tmem_relinquish_pair();
     }
-    if (warp == 0 && p.offsets) {                        // the table of tiles
-        int before = 0;
-        for (int e0 = 0; e0 < p.experts; e0 += 32) {
-            const int e = e0 + lane;
-            int64_t a = 0, b = 0;
-            if (e < p.experts) { a = first_row(p, e); b = first_row(p, e + 1); }
-            const int tiles = b > a ? token_tiles(b - a) * p.tiles_c : 0;
-            int scan = tiles;
-#pragma unroll
-            for (int d = 1; d < 32; d *= 2) {
-                const int up = __shfl_up_sync(0xffffffffu, scan, d);
-                if (lane >= d) scan += up;
-            }
-            if (e < p.experts) {
-                first_s[e] = before + scan - tiles;
-                row_s[e] = (int32_t)a;
-                if (e == p.experts - 1) { first_s[e + 1] = before + scan; row_s[e + 1] = (int32_t)b; }
-            }
-            before += __shfl_sync(0xffffffffu, scan, 31);
-        }
-    }
+    if (warp == 0 && p.offsets) make_table(p, first_s, row_s, [](int64_t n) { return token_tiles(n); });
     tc::tc_fence_before();
     __syncthreads();
     tc::cluster_sync_all();                              // the other CTA's barriers exist before anything targets them
@@ -575,33 +639,18 @@ w8a8_pair_kernel(const __grid_constant__ PairMaps maps, const Params p, int band
     } else {
         const int quarter = warp & 3, c = quarter * 32 + lane;                   // tcgen05.ld: a warp reads lanes 32 * (warp % 4) ...
         const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
-        if (p.offsets)                                                           // rows behind the last expert's
-            for (int64_t r = row_s[p.experts] + (int64_t)blockIdx.x; r < p.rows; r += gridDim.x)
-                for (int64_t i = tid - 64; i < p.N; i += THREADS - 64) {
-                    if constexpr (GATED) reinterpret_cast<float*>(p.y)[r * p.N + i] = 0.f;
-                    else reinterpret_cast<uint16_t*>(p.y)[r * p.N + i] = 0;
-                }
+        if (p.offsets) zero_tail<GATED>(p, row_s[p.experts], tid - 64);
         uint32_t ab = 0, aphase = 0;
         bool ok = true;
         for (int t = pair; t < n_tiles; t += n_pairs) {
             const Tile tile = order.at(t);
-            Lane L;
-            L.row0 = tile.row0;
-            L.n_rows = tile.n_rows;
-            L.n = (int64_t)tile.ct * 2 * WIDTH + rank * WIDTH + (GATED ? c >> 1 : c);
-            L.sw = 0.f;
-            L.bias = 0.f;
-            if (L.n < p.N) {
-                L.sw = p.ws[(int64_t)tile.expert * (GATED ? 2 * p.N : p.N) + L.n + (GATED && (c & 1) ? p.N : 0)];
-                if (!GATED && p.bias) L.bias = p.bias[L.n];
-            }
             float* sx = sx_s + ab * PAIR_TOKENS;
+            const Lane L = make_lane<GATED>(p, tile, (int64_t)tile.ct * 2 * WIDTH + rank * WIDTH, c, sx);
             for (int i = tid - 64; i < tile.nt; i += THREADS - 64) sx[i] = i < tile.n_rows ? p.xs[tile.row0 + i] : 0.f;
             asm volatile("bar.sync 1, 128;" ::: "memory");                       // the epilogue's own barrier
-            L.sx = sx;
             if (ok) ok = __all_sync(0xffffffffu, tc::mbar_wait(&acc_full[ab], aphase));
             tc::tc_fence_after();
-            const int chunks = ok ? tile.nt / 32 : 0;        // after a give-up: no more work, but every barrier of the warps
+            const int chunks = ok ? tile.nt / 32 : 0;                            // after a give-up: no more work, but every barrier of the warps
 #pragma unroll 1
             for (int c0 = 0; c0 < chunks; ++c0) {
                 uint32_t v[32];
@@ -612,9 +661,7 @@ w8a8_pair_kernel(const __grid_constant__ PairMaps maps, const Params p, int band
                     __syncwarp();
                     if (lane == 0) tc::mbar_arrive_cluster(tc::map_to_rank(&acc_empty[ab], 0));
                 }
-#pragma unroll
-                for (int j = 0; j < 32; j += 2)
-                    if (c0 * 32 + j < tile.n_rows) emit_pair<GATED>(p, L, c0 * 32 + j, v[j], v[j + 1]);
+                emit<GATED, 32>(p, L, c0 * 32, v);
             }
             if (++ab == PAIR_ACC) { ab = 0; aphase ^= 1; }
         }
@@ -659,39 +706,43 @@ int make_token_map(CUtensorMap* map, const W8A8Problem& p, int box_rows)
     return WUSH_OK;
 }
 
+// Upper bound of the tiles of a launch.
+int64_t stream_tiles(const W8A8Problem& w, int nt)
+{
+    const int64_t slots = (w.rows + nt - 1) / nt + (w.offsets ? std::min(w.experts, w.rows) : 0), width = w.gated ? 64 : 128;
+    return slots * ((w.N + width - 1) / width);
+}
+
 template <int NT, bool GATED>
-int launch_small(const W8A8Problem& w, Params p, int64_t slots, int split, bool dependent, cudaStream_t st)
+int launch_stream(const W8A8Problem& w, Params p, bool dependent, cudaStream_t st)
 {
     CUtensorMap mw, mx;
     if (int e = make_weight_map(&mw, w)) return e;
     if (int e = make_token_map(&mx, w, NT)) return e;
-    const int64_t grid = slots * p.tiles_c * split;
-    if (grid > 0x7fffffffll) return fail(WUSH_ERR_UNSUPPORTED, "w8a8: too many tiles (%lld)", (long long)grid);
+    p.tiles_c = (int)((w.N + (GATED ? 63 : 127)) / (GATED ? 64 : 128));
+    const int64_t most = stream_tiles(w, NT);
+    if (most * ((w.K + 127) / 128) > 0x7fffffffll) return fail(WUSH_ERR_UNSUPPORTED, "w8a8: too many tiles (%lld)", (long long)most);
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)grid);
+    cfg.gridDim = dim3((unsigned)sm_count());
     cfg.blockDim = dim3(THREADS);
-    cfg.dynamicSmemBytes = Small<NT>::SMEM;
+    cfg.dynamicSmemBytes = Stream<NT>::SMEM;
     cfg.stream = st;
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = split;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = dependent ? 2 : 1;
-    cudaError_t e = cudaLaunchKernelEx(&cfg, w8a8_small_kernel<NT, GATED>, mw, mx, p);
+    cfg.numAttrs = dependent ? 1 : 0;
+    cudaError_t e = cudaLaunchKernelEx(&cfg, w8a8_stream_kernel<NT, GATED>, mw, mx, p);
     if (e != cudaSuccess) return fail(WUSH_ERR_CUDA, "w8a8: launch failed: %s", cudaGetErrorString(e));
     return WUSH_OK;
 }
 
 template <int NT>
-int set_small()
+int set_stream()
 {
-    cudaError_t e = cudaFuncSetAttribute(w8a8_small_kernel<NT, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, Small<NT>::SMEM);
+    cudaError_t e = cudaFuncSetAttribute(w8a8_stream_kernel<NT, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, Stream<NT>::SMEM);
     if (e == cudaSuccess)
-        e = cudaFuncSetAttribute(w8a8_small_kernel<NT, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, Small<NT>::SMEM);
+        e = cudaFuncSetAttribute(w8a8_stream_kernel<NT, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, Stream<NT>::SMEM);
     if (e != cudaSuccess) return fail(WUSH_ERR_CUDA, "w8a8: cudaFuncSetAttribute failed: %s", cudaGetErrorString(e));
     return WUSH_OK;
 }
@@ -758,22 +809,21 @@ int set_pair()
     return WUSH_OK;
 }
 
-// CTAs along K of one tile: doubled while the launch has less than `want` CTAs and each keeps four stages of K or more.
-int pick_split(int64_t tiles, int k_steps, int nt, int64_t want)
-{
-    int s = 1;
-    while (s < MAX_SPLIT && nt / (2 * s) >= 2 && tiles * s < want && k_steps / (2 * s) >= 4) s *= 2;
-    return s;
-}
-
 }  // namespace
+
+// Token columns of the streaming kernel's tiles, 0 for the pair kernel: by the mean number of rows of an expert.
+static int stream_tokens(int64_t rows, int64_t experts)
+{
+    const int64_t groups = std::min(experts, rows), per = groups ? (rows + groups - 1) / groups : 0;
+    return per <= 16 ? 16 : per <= 32 ? 32 : per <= 64 ? 64 : 0;
+}
 
 int w8a8_set_attributes()
 {
     if (int s = resolve_tensor_map_encoder()) return s;
-    if (int s = set_small<16>()) return s;
-    if (int s = set_small<32>()) return s;
-    if (int s = set_small<64>()) return s;
+    if (int s = set_stream<16>()) return s;
+    if (int s = set_stream<32>()) return s;
+    if (int s = set_stream<64>()) return s;
     if (int s = set_pair()) return s;
     return WUSH_OK;
 }
@@ -787,7 +837,14 @@ int w8a8_take_error(int* word)
     return e == cudaSuccess ? WUSH_OK : fail(WUSH_ERR_CUDA, "device_flag(w8a8): %s", cudaGetErrorString(e));
 }
 
-int w8a8_launch(const W8A8Problem& w, bool dependent, cudaStream_t st)
+// Counters, then the slots of the streaming kernel; 0 where the pairs run.
+size_t w8a8_workspace_bytes(int64_t rows, int64_t experts)
+{
+    const int nt = stream_tokens(rows, experts);
+    return nt ? W8A8_COUNTER_BYTES + (size_t)2 * sm_count() * 128 * nt * sizeof(int32_t) : 0;
+}
+
+int w8a8_launch(const W8A8Problem& w, void* workspace, bool dependent, cudaStream_t st)
 {
     if (w.rows == 0 || w.N == 0) return WUSH_OK;
     Params p = {};
@@ -795,18 +852,15 @@ int w8a8_launch(const W8A8Problem& w, bool dependent, cudaStream_t st)
     p.rows = w.rows; p.N = w.N; p.K = (int)w.K; p.experts = (int)w.experts;
     p.bf16_out = w.out_dtype == WUSH_BF16;
     p.early = dependent ? 1 : 0;
-    const int width = w.gated ? 64 : 128;
-    p.tiles_c = (int)((w.N + width - 1) / width);
-    const int64_t groups = std::min(w.experts, w.rows), per = (w.rows + groups - 1) / groups;
-    if (per > 64) return w.gated ? launch_pair<true>(w, p, dependent, st) : launch_pair<false>(w, p, dependent, st);
-    const int nt = per <= 16 ? 16 : per <= 32 ? 32 : 64;
-    const int64_t slots = w.offsets ? w.rows / nt + groups : (w.rows + nt - 1) / nt;
-    const int split = pick_split(slots * p.tiles_c, (int)((w.K + 127) / 128), nt, 8 * sm_count());
-#define WUSH_SMALL(NT) return w.gated ? launch_small<NT, true>(w, p, slots, split, dependent, st) : launch_small<NT, false>(w, p, slots, split, dependent, st)
-    if (nt == 16) WUSH_SMALL(16);
-    if (nt == 32) WUSH_SMALL(32);
-    WUSH_SMALL(64);
-#undef WUSH_SMALL
+    const int nt = stream_tokens(w.rows, w.experts);
+    if (nt == 0) return w.gated ? launch_pair<true>(w, p, dependent, st) : launch_pair<false>(w, p, dependent, st);
+    p.counters = (int32_t*)workspace;
+    p.pieces = (uint32_t*)((uint8_t*)workspace + W8A8_COUNTER_BYTES);
+#define WUSH_STREAM(NT) return w.gated ? launch_stream<NT, true>(w, p, dependent, st) : launch_stream<NT, false>(w, p, dependent, st)
+    if (nt == 16) WUSH_STREAM(16);
+    if (nt == 32) WUSH_STREAM(32);
+    WUSH_STREAM(64);
+#undef WUSH_STREAM
 }
 
 }  // namespace wush
@@ -830,8 +884,32 @@ int check_product(const char* op, const wush::W8A8Problem& p)
 }
 }  // namespace
 
+// A product on its own: the counters of the workspace are zeroed by a memset in front (in the calls below that chain
+// kernels, by the first of them).
+namespace {
+int launch_alone(const char* op, const wush::W8A8Problem& p, void* workspace, size_t workspace_bytes, cudaStream_t st)
+{
+    using namespace wush;
+    const size_t need = w8a8_workspace_bytes(p.rows, p.experts);
+    if (need) {
+        if (!workspace || workspace_bytes < need)
+            return fail(WUSH_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, %zu given", op, need, workspace ? workspace_bytes : (size_t)0);
+        WUSH_REQUIRE(aligned16(workspace), "%s: the workspace must be 16-byte aligned", op);
+        cudaError_t e = cudaMemsetAsync(workspace, 0, W8A8_COUNTER_BYTES, st);
+        if (e != cudaSuccess) return fail(WUSH_ERR_CUDA, "%s: cudaMemsetAsync: %s", op, cudaGetErrorString(e));
+    }
+    return w8a8_launch(p, workspace, false, st);
+}
+}  // namespace
+
+WUSH_API size_t wush_w8a8_gemm_workspace_bytes(int64_t M, int64_t experts)
+{
+    if (M <= 0 || experts <= 0) return 0;
+    return wush::w8a8_workspace_bytes(M, experts);
+}
+
 WUSH_API int wush_w8a8_gemm(const int8_t* xq, const float* xs, const int8_t* wq, const float* ws, const float* bias, int64_t M, int64_t N,
-                            int64_t K, void* y, int out_dtype, void* stream)
+                            int64_t K, void* y, int out_dtype, void* workspace, size_t workspace_bytes, void* stream)
 {
     using namespace wush;
     WUSH_REQUIRE(out_dtype == WUSH_F16 || out_dtype == WUSH_BF16, "w8a8_gemm: the result is fp16 or bf16");
@@ -839,11 +917,12 @@ WUSH_API int wush_w8a8_gemm(const int8_t* xq, const float* xs, const int8_t* wq,
     if (int e = check_product("w8a8_gemm", p)) return e;
     if (M == 0 || N == 0) return WUSH_OK;
     if (int e = ensure_init()) return e;
-    return w8a8_launch(p, false, (cudaStream_t)stream);
+    return launch_alone("w8a8_gemm", p, workspace, workspace_bytes, (cudaStream_t)stream);
 }
 
 WUSH_API int wush_w8a8_grouped_gemm(const int8_t* xq, const float* xs, const int8_t* wq, const float* ws, const int32_t* offsets,
-                                    int64_t rows, int64_t experts, int64_t N, int64_t K, void* y, int out_dtype, void* stream)
+                                    int64_t rows, int64_t experts, int64_t N, int64_t K, void* y, int out_dtype, void* workspace,
+                                    size_t workspace_bytes, void* stream)
 {
     using namespace wush;
     WUSH_REQUIRE(out_dtype == WUSH_F16 || out_dtype == WUSH_BF16, "w8a8_grouped_gemm: the result is fp16 or bf16");
@@ -852,11 +931,12 @@ WUSH_API int wush_w8a8_grouped_gemm(const int8_t* xq, const float* xs, const int
     if (rows == 0 || N == 0) return WUSH_OK;
     WUSH_REQUIRE(offsets, "w8a8_grouped_gemm: null pointer");
     if (int e = ensure_init()) return e;
-    return w8a8_launch(p, false, (cudaStream_t)stream);
+    return launch_alone("w8a8_grouped_gemm", p, workspace, workspace_bytes, (cudaStream_t)stream);
 }
 
 WUSH_API int wush_w8a8_grouped_gated(const int8_t* xq, const float* xs, const int8_t* wq, const float* ws, const int32_t* offsets,
-                                     int64_t rows, int64_t experts, int64_t I, int64_t K, float* h, void* stream)
+                                     int64_t rows, int64_t experts, int64_t I, int64_t K, float* h, void* workspace, size_t workspace_bytes,
+                                     void* stream)
 {
     using namespace wush;
     const W8A8Problem p = {xq, xs, wq, ws, nullptr, offsets, rows, I, K, experts, true, WUSH_F32, h};
@@ -864,34 +944,48 @@ WUSH_API int wush_w8a8_grouped_gated(const int8_t* xq, const float* xs, const in
     if (rows == 0 || I == 0) return WUSH_OK;
     WUSH_REQUIRE(offsets, "w8a8_grouped_gated: null pointer");
     if (int e = ensure_init()) return e;
-    return w8a8_launch(p, false, (cudaStream_t)stream);
+    return launch_alone("w8a8_grouped_gated", p, workspace, workspace_bytes, (cudaStream_t)stream);
 }
 
 // Activations to codes, then the product: two launches, the second fetching its first weights under the first.
+namespace {
+struct LinearPlan {
+    size_t xq, xs, total;        // the product's workspace comes first
+};
+LinearPlan linear_plan(int64_t M, int64_t K)
+{
+    LinearPlan f = {};
+    f.xq = (wush::w8a8_workspace_bytes(M, 1) + 255) & ~(size_t)255;
+    f.xs = f.xq + (((size_t)(M * K) + 255) & ~(size_t)255);
+    f.total = f.xs + (size_t)M * 4;
+    return f;
+}
+}  // namespace
 WUSH_API size_t wush_w8a8_linear_workspace_bytes(int64_t M, int64_t K)
 {
-    if (M <= 0 || K <= 0) return 0;
-    return (size_t)(((M * K + 255) & ~255ll) + M * 4);
+    return M <= 0 || K <= 0 ? 0 : linear_plan(M, K).total;
 }
 WUSH_API int wush_w8a8_linear(const void* x, int dtype, const int8_t* wq, const float* ws, const float* bias, int64_t M, int64_t N, int64_t K,
                               void* y, void* workspace, size_t workspace_bytes, void* stream)
 {
     using namespace wush;
     WUSH_REQUIRE(dtype == WUSH_F16 || dtype == WUSH_BF16, "w8a8_linear: activations are fp16 or bf16");
-    int8_t* xq = (int8_t*)workspace;
-    float* xs = (float*)(xq + ((M * K + 255) & ~255ll));
+    const LinearPlan f = linear_plan(M > 0 ? M : 0, K > 0 ? K : 0);
+    int8_t* xq = (int8_t*)workspace + f.xq;
+    float* xs = (float*)((uint8_t*)workspace + f.xs);
     const W8A8Problem p = {xq, xs, wq, ws, bias, nullptr, M, N, K, 1, false, dtype, y};
     if (M > 0 && N > 0) {
-        if (!workspace || workspace_bytes < wush_w8a8_linear_workspace_bytes(M, K))
-            return fail(WUSH_ERR_WORKSPACE, "w8a8_linear: workspace of %zu bytes needed, %zu given",
-                        wush_w8a8_linear_workspace_bytes(M, K), workspace ? workspace_bytes : (size_t)0);
+        if (!workspace || workspace_bytes < f.total)
+            return fail(WUSH_ERR_WORKSPACE, "w8a8_linear: workspace of %zu bytes needed, %zu given", f.total,
+                        workspace ? workspace_bytes : (size_t)0);
         WUSH_REQUIRE(x && aligned16(x), "w8a8_linear: x must be a 16-byte aligned pointer");
     }
     if (int e = check_product("w8a8_linear", p)) return e;
     if (M == 0 || N == 0) return WUSH_OK;
     if (int e = ensure_init()) return e;
-    if (int e = quant_int8_launch(x, dtype, M, K, xq, xs, nullptr, 1, nullptr, false, (cudaStream_t)stream)) return e;
-    return w8a8_launch(p, true, (cudaStream_t)stream);
+    const QuantRows q = {x, dtype, M, K, xq, xs, nullptr, 1, nullptr, w8a8_workspace_bytes(M, 1) ? (int32_t*)workspace : nullptr};
+    if (int e = quant_int8_launch(q, false, (cudaStream_t)stream)) return e;
+    return w8a8_launch(p, workspace, true, (cudaStream_t)stream);
 }
 
 // ---- the expert block ----------------------------------------------------------------------------------------------------
@@ -901,7 +995,7 @@ WUSH_API int wush_w8a8_linear(const void* x, int dtype, const int8_t* wq, const 
 namespace {
 struct FfnPlan {
     int64_t R;
-    size_t pos, offsets, xq, xs, h, hq, hs, o, total;
+    size_t up, down, pos, offsets, xq, xs, h, hq, hs, o, total;
 };
 FfnPlan ffn_plan(int64_t T, int64_t H, int64_t I, int64_t E, int64_t k)
 {
@@ -909,6 +1003,8 @@ FfnPlan ffn_plan(int64_t T, int64_t H, int64_t I, int64_t E, int64_t k)
     f.R = T * k;
     size_t at = 0;
     auto take = [&](size_t bytes) { const size_t here = at; at += (bytes + 255) & ~(size_t)255; return here; };
+    f.up = take(wush::w8a8_workspace_bytes(f.R, E));
+    f.down = take(wush::w8a8_workspace_bytes(f.R, E));
     f.pos = take(f.R * 4);
     f.offsets = take((E + 1) * 4);
     f.xq = take(f.R * H);
@@ -958,9 +1054,12 @@ WUSH_API int wush_w8a8_expert_ffn(const void* x, int dtype, const void* ids, int
     if (int e = ensure_init()) return e;
     cudaStream_t st = (cudaStream_t)stream;
     if (int e = expert_sort_launch(ids, id_bytes, f.R, (int)experts, pos, offsets, st)) return e;
-    if (int e = quant_int8_launch(x, dtype, tokens, H, xq, xs, pos, (int)k, offsets + experts, true, st)) return e;
-    if (int e = w8a8_launch(up, true, st)) return e;
-    if (int e = quant_int8_launch(h, WUSH_F32, f.R, I, hq, hs, nullptr, 1, nullptr, true, st)) return e;
-    if (int e = w8a8_launch(down, true, st)) return e;
+    const bool counted = w8a8_workspace_bytes(f.R, experts) != 0;       // both products of a block run on the same kernel
+    const QuantRows qx = {x, dtype, tokens, H, xq, xs, pos, (int)k, offsets + experts, counted ? (int32_t*)(base + f.up) : nullptr};
+    const QuantRows qh = {h, WUSH_F32, f.R, I, hq, hs, nullptr, 1, nullptr, counted ? (int32_t*)(base + f.down) : nullptr};
+    if (int e = quant_int8_launch(qx, true, st)) return e;
+    if (int e = w8a8_launch(up, base + f.up, true, st)) return e;
+    if (int e = quant_int8_launch(qh, true, st)) return e;
+    if (int e = w8a8_launch(down, base + f.down, true, st)) return e;
     return expert_combine_launch(base + f.o, dtype, tokens, H, pos, (int)k, weights, y, true, st);
 }

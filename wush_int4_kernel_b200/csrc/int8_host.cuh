@@ -23,8 +23,18 @@ static inline int check_entries(const char* op, int64_t tokens, int64_t k, int64
 // Launchers used by the entry points of one operator and by the expert block, which chains them.  `dependent`: launched
 // with programmatic serialisation, so the kernel may start under the one before it; it waits for that one before it reads
 // anything that a kernel wrote.
-int quant_int8_launch(const void* x, int dtype, int64_t rows, int64_t K, int8_t* q, float* s, const int32_t* pos, int k,
-                      const int32_t* n_used, bool dependent, cudaStream_t st);
+struct QuantRows {
+    const void* x;
+    int dtype;
+    int64_t rows, K;
+    int8_t* q;
+    float* s;
+    const int32_t* pos;      // (rows, k) destinations, or null: row r to row r
+    int k;
+    const int32_t* n_used;   // with pos: rows of the result from *n_used on become zero
+    int32_t* counters;       // W8A8_COUNTER_BYTES to zero for the product that follows, or null
+};
+int quant_int8_launch(const QuantRows& a, bool dependent, cudaStream_t st);
 int expert_sort_launch(const void* ids, int id_bytes, int64_t n, int n_experts, int32_t* pos, int32_t* offsets, cudaStream_t st);
 int expert_combine_launch(const void* rows, int dtype, int64_t tokens, int64_t H, const int32_t* pos, int k, const float* weights,
                           void* y, bool dependent, cudaStream_t st);
@@ -41,6 +51,9 @@ struct W8A8Problem {
     int out_dtype;           // gated: always fp32
     void* y;                 // (rows, N)
 };
-int w8a8_launch(const W8A8Problem& p, bool dependent, cudaStream_t st);
+// The product's workspace: counters, which are zero when its kernel starts, then slots.
+constexpr size_t W8A8_COUNTER_BYTES = 1024;
+size_t w8a8_workspace_bytes(int64_t rows, int64_t experts);
+int w8a8_launch(const W8A8Problem& p, void* workspace, bool dependent, cudaStream_t st);
 
 }  // namespace wush

@@ -118,11 +118,13 @@ template <typename T>
 __global__ void __launch_bounds__(1024) quant_int8_kernel(const T* __restrict__ x, int64_t rows, int K, int tpr,
                                                           int8_t* __restrict__ q, float* __restrict__ s,
                                                           const int32_t* __restrict__ pos, int k,
-                                                          const int32_t* __restrict__ n_used)
+                                                          const int32_t* __restrict__ n_used, int32_t* __restrict__ counters)
 {
     pdl_wait();
     pdl_launch_dependents();
     __shared__ uint32_t part[32];
+    if (counters && blockIdx.x == 0)
+        for (int i = threadIdx.x; i < (int)(W8A8_COUNTER_BYTES / 4); i += blockDim.x) counters[i] = 0;
     const int group = threadIdx.x / tpr, lane = threadIdx.x - group * tpr;
     const int64_t row = (int64_t)blockIdx.x * (blockDim.x / tpr) + group;
     const int vecs = K / VEC;
@@ -191,36 +193,34 @@ __global__ void __launch_bounds__(1024) quant_int8_kernel(const T* __restrict__ 
 }
 
 template <typename T>
-int launch_quant(const void* x, int64_t rows, int64_t K, int8_t* q, float* s, const int32_t* pos, int k, const int32_t* n_used,
-                 bool dependent, cudaStream_t st)
+int launch_quant(const QuantRows& a, bool dependent, cudaStream_t st)
 {
-    const int vecs = (int)(K / VEC);
+    const int vecs = (int)(a.K / VEC);
     // Few rows: a thread for every 16 elements.  Many: two steps per thread, which the registers hold.
-    const int want = rows <= 2 * sm_count() ? vecs : (vecs + HOLD - 1) / HOLD;
+    const int want = a.rows <= 2 * sm_count() ? vecs : (vecs + HOLD - 1) / HOLD;
     int tpr = 32;
     while (tpr < want && tpr < 1024) tpr *= 2;
     const int block = tpr < 256 ? 256 : tpr;
-    const int64_t per = block / tpr, grid = (rows + per - 1) / per;
-    if (grid > 0x7fffffffll) return fail(WUSH_ERR_UNSUPPORTED, "quant_int8: too many rows (%lld)", (long long)rows);
+    const int64_t per = block / tpr, grid = (a.rows + per - 1) / per;
+    if (grid > 0x7fffffffll) return fail(WUSH_ERR_UNSUPPORTED, "quant_int8: too many rows (%lld)", (long long)a.rows);
     if (dependent) {
-        cudaError_t e = launch_dependent(quant_int8_kernel<T>, dim3((unsigned)grid), dim3(block), 0, st, (const T*)x, rows, (int)K,
-                                         tpr, q, s, pos, k, n_used);
+        cudaError_t e = launch_dependent(quant_int8_kernel<T>, dim3((unsigned)grid), dim3(block), 0, st, (const T*)a.x, a.rows, (int)a.K,
+                                         tpr, a.q, a.s, a.pos, a.k, a.n_used, a.counters);
         if (e != cudaSuccess) return fail(WUSH_ERR_CUDA, "quant_int8: launch failed: %s", cudaGetErrorString(e));
         return WUSH_OK;
     }
-    quant_int8_kernel<T><<<(unsigned)grid, block, 0, st>>>((const T*)x, rows, (int)K, tpr, q, s, pos, k, n_used);
+    quant_int8_kernel<T><<<(unsigned)grid, block, 0, st>>>((const T*)a.x, a.rows, (int)a.K, tpr, a.q, a.s, a.pos, a.k, a.n_used, a.counters);
     return check_launch("quant_int8");
 }
 
 }  // namespace
 
-int quant_int8_launch(const void* x, int dtype, int64_t rows, int64_t K, int8_t* q, float* s, const int32_t* pos, int k,
-                      const int32_t* n_used, bool dependent, cudaStream_t st)
+int quant_int8_launch(const QuantRows& a, bool dependent, cudaStream_t st)
 {
-    switch (dtype) {
-        case WUSH_BF16: return launch_quant<__nv_bfloat16>(x, rows, K, q, s, pos, k, n_used, dependent, st);
-        case WUSH_F16: return launch_quant<__half>(x, rows, K, q, s, pos, k, n_used, dependent, st);
-        default: return launch_quant<float>(x, rows, K, q, s, pos, k, n_used, dependent, st);
+    switch (a.dtype) {
+        case WUSH_BF16: return launch_quant<__nv_bfloat16>(a, dependent, st);
+        case WUSH_F16: return launch_quant<__half>(a, dependent, st);
+        default: return launch_quant<float>(a, dependent, st);
     }
 }
 
@@ -236,7 +236,7 @@ WUSH_API int wush_quant_int8(const void* x, int dtype, int64_t rows, int64_t K, 
     WUSH_REQUIRE(x && q && s, "quant_int8: null pointer");
     WUSH_REQUIRE(aligned16(x) && aligned16(q) && aligned4(s), "quant_int8: x and q must be 16-byte aligned, s 4-byte");
     if (int e = ensure_init()) return e;
-    return quant_int8_launch(x, dtype, rows, K, q, s, nullptr, 1, nullptr, false, (cudaStream_t)stream);
+    return quant_int8_launch({x, dtype, rows, K, q, s, nullptr, 1, nullptr, nullptr}, false, (cudaStream_t)stream);
 }
 
 WUSH_API int wush_expert_gather_quant_int8(const void* x, int dtype, int64_t tokens, int64_t K, const int32_t* pos, int64_t k,
@@ -252,5 +252,5 @@ WUSH_API int wush_expert_gather_quant_int8(const void* x, int dtype, int64_t tok
     WUSH_REQUIRE(aligned16(x) && aligned16(q) && aligned4(s) && aligned4(pos) && aligned4(offsets),
                  "expert_gather_quant_int8: x and q must be 16-byte aligned, s, pos and offsets 4-byte");
     if (int e = ensure_init()) return e;
-    return quant_int8_launch(x, dtype, tokens, K, q, s, pos, (int)k, offsets + n_experts, false, (cudaStream_t)stream);
+    return quant_int8_launch({x, dtype, tokens, K, q, s, pos, (int)k, offsets + n_experts, nullptr}, false, (cudaStream_t)stream);
 }
