@@ -39,8 +39,11 @@ template <int NT> struct Stream {
     static constexpr int STAGE = A_BYTES + NT * 128;
     static constexpr int TABLE_BYTES = 2 * (WUSH_EXPERT_MAX + 2) * 4;
     static constexpr int FIXED = 2 * NT * 4 + TABLE_BYTES + 256 + 1024;
-    static constexpr int STAGES = (226 * 1024 - FIXED) / STAGE;
+    // Eight stages: 128 KB of weights in flight.  More is slower (470 MB: 83.6 us with twelve, 79.3 with eight, 80.9 with
+    // six): a copy loop of nothing but these loads shows the same, 76 us with twelve and 74 with six.
+    static constexpr int STAGES = 8;
     static constexpr int SMEM = STAGES * STAGE + FIXED;
+    static_assert(SMEM <= 227 * 1024, "shared memory of a CTA");
     static constexpr int COLS = 2 * NT < 32 ? 32 : 2 * NT;           // columns of tensor memory: two accumulators
     static constexpr int PIECE = 128 * NT;                           // sums of a tile
 };
@@ -55,7 +58,7 @@ struct Params {
     int K, experts, tiles_c;     // tiles_c: channel tiles
     int bf16_out;
     int early;                   // weights (and offsets) may be read before the kernel in front has finished
-    int32_t* counters;           // one per CTA, zero; null: no tile is split
+    int32_t* counters;           // one per CTA, zero
     uint32_t* pieces;            // two per CTA
 };
 
@@ -70,12 +73,20 @@ __device__ __forceinline__ uint64_t desc_sw128(uint32_t saddr)
     return d;
 }
 
-__device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1, int c2, int c3)
+// Weights that pass once: the lines leave L2 first, so that the activations stay (470 MB with one token: 79.3 -> 78.2 us,
+// with 64 tokens: 88.8 -> 85.1 us).
+__device__ __forceinline__ uint64_t evict_first_policy()
+{
+    uint64_t policy;
+    asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
+    return policy;
+}
+__device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1, int c2, int c3, uint64_t policy)
 {
     asm volatile(
-        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%3, %4, %5, %6}], [%2], %7;" ::"r"(
             tc::smem_u32(dst)),
-        "l"(map), "r"(tc::smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+        "l"(map), "r"(tc::smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "l"(policy)
         : "memory");
 }
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* r)
@@ -222,25 +233,50 @@ __device__ __forceinline__ void zero_tail(const Params& p, int64_t used, int tid
 // Runs end at tile borders where that costs no more than FIXUP_STAGES stages of balance; otherwise they are of equal length,
 // and a tile cut by a border is finished by whichever of its CTAs comes last: every CTA leaves its sums in a slot of the
 // workspace and counts itself in, and the last one adds the slots (int32: in any order the same sum).  Nobody waits.
+// A CTA takes its two cut tiles first and whole tiles after them, so that the cut ones are finished while others stream
+// (4096 x 24576, 1 token: 24.3 -> ORDER_US us).
 constexpr int FIXUP_STAGES = 8;
 
 struct Run {
     int64_t begin, end;          // stages of this CTA
     int64_t total;
     int ctas;                    // CTAs that have a run
-    bool split;
+    int k_steps;
+    int pieces;                  // tiles and parts of tiles in the run
+    bool head, tail;             // begins inside a tile; ends inside another one
 };
 __device__ __forceinline__ Run make_run(const Params& p, int64_t tiles, int k_steps, int cta, int ctas)
 {
     Run r;
     r.total = tiles * k_steps;
+    r.k_steps = k_steps;
     const int64_t whole = (tiles + ctas - 1) / ctas * k_steps, even = (r.total + ctas - 1) / ctas + FIXUP_STAGES;
-    r.split = p.counters && whole > even;
-    r.ctas = r.split ? (int)min((int64_t)ctas, r.total) : ctas;
+    const bool split = whole > even;
+    r.ctas = split ? (int)min((int64_t)ctas, r.total) : ctas;
     if (cta >= r.ctas) r.begin = r.end = 0;
-    else if (r.split) { r.begin = r.total * cta / r.ctas; r.end = r.total * (cta + 1) / r.ctas; }
+    else if (split) { r.begin = r.total * cta / r.ctas; r.end = r.total * (cta + 1) / r.ctas; }
     else { r.begin = tiles * cta / ctas * k_steps; r.end = tiles * (cta + 1) / ctas * k_steps; }
+    const int64_t first = r.begin / k_steps, last = (r.end + k_steps - 1) / k_steps;
+    r.pieces = r.end > r.begin ? (int)(last - first) : 0;
+    r.head = r.begin % k_steps != 0;
+    r.tail = r.end % k_steps != 0 && (r.pieces > 1 || !r.head);
     return r;
+}
+// Piece i of a run: stages [k0, k1) of tile t.
+struct Piece {
+    int t, k0, k1;
+};
+__device__ __forceinline__ Piece piece_of(const Run& r, int i)
+{
+    const int first = (int)(r.begin / r.k_steps), last = (int)((r.end - 1) / r.k_steps);
+    Piece q;
+    if (r.head && i == 0) q.t = first;
+    else if (r.tail && i == (r.head ? 1 : 0)) q.t = last;
+    else q.t = first + i - (r.tail ? 1 : 0);
+    const int64_t start = (int64_t)q.t * r.k_steps;
+    q.k0 = (int)max((int64_t)0, r.begin - start);
+    q.k1 = (int)min((int64_t)r.k_steps, r.end - start);
+    return q;
 }
 // The CTA of a split whose run holds `stage`: the last one that begins at or before it.
 __device__ __forceinline__ int owner(const Run& r, int64_t stage) { return (int)(((stage + 1) * r.ctas - 1) / r.total); }
@@ -259,6 +295,7 @@ struct StreamOrder {
         int local = t;
         if (first) {
             while (t >= first[e + 1]) ++e;
+            while (t < first[e]) --e;
             start = row[e];
             count = row[e + 1] - row[e];
             local = t - first[e];
@@ -318,40 +355,43 @@ __global__ void __launch_bounds__(THREADS, 1) w8a8_stream_kernel(const __grid_co
 
     if (warp == 0) {
         if (lane == 0) {
+            const uint64_t policy = evict_first_policy();
             const int n = (int)(run.end - run.begin);
-            int t = n ? (int)(run.begin / k_steps) : 0, ks = n ? (int)(run.begin - (int64_t)t * k_steps) : 0;
+            int i = 0, ks = 0;                                           // current piece and stage
+            Piece q = {};
             Tile tile = {};
-            if (n) tile = order.at(t);
-            const int t_first = t, ks_first = ks;
-            auto step = [&](bool more) {
-                if (++ks == k_steps) { ks = 0; ++t; if (more) tile = order.at(t); }
+            auto start = [&](int piece) {
+                i = piece;
+                q = piece_of(run, i);
+                tile = order.at(q.t);
+                ks = q.k0;
+            };
+            auto step = [&]() {
+                if (++ks == q.k1 && i + 1 < run.pieces) start(i + 1);
             };
             const int ahead = n < C::STAGES ? n : C::STAGES;
-            for (int i = 0; i < ahead; ++i) {                            // the weights do not depend on the kernel in front
-                tc::mbar_expect_tx(&full[i], C::STAGE);
-                tma_load_4d(smem + i * C::STAGE, &map_w, &full[i], ks * 128, 0, tile.ct * WIDTH, tile.expert);
-                step(i + 1 < n);
+            if (n) start(0);
+            for (int j = 0; j < ahead; ++j) {                            // the weights do not depend on the kernel in front
+                tc::mbar_expect_tx(&full[j], C::STAGE);
+                tma_load_4d(smem + j * C::STAGE, &map_w, &full[j], ks * 128, 0, tile.ct * WIDTH, tile.expert, policy);
+                step();
             }
-            const int t_next = t, ks_next = ks;
             if (p.early) pdl_wait();
-            if (n) { order.e = 0; t = t_first; ks = ks_first; tile = order.at(t); }
-            for (int i = 0; i < ahead; ++i) {
-                tc::tma_load_2d(smem + i * C::STAGE + A_BYTES, &map_x, &full[i], ks * 128, (int)tile.row0);
-                step(i + 1 < n);
+            if (n) start(0);
+            for (int j = 0; j < ahead; ++j) {
+                tc::tma_load_2d(smem + j * C::STAGE + A_BYTES, &map_x, &full[j], ks * 128, (int)tile.row0);
+                step();
             }
-            t = t_next;
-            ks = ks_next;
             int issued = ahead;
             uint32_t s = 0, phase = 0;
             bool ok = true;
-            for (int i = ahead; i < n; ++i) {
+            for (; issued < n; ++issued) {
                 if (!tc::mbar_wait(&empty[s], phase)) { ok = false; break; }
                 tc::mbar_expect_tx(&full[s], C::STAGE);
-                tma_load_4d(smem + s * C::STAGE, &map_w, &full[s], ks * 128, 0, tile.ct * WIDTH, tile.expert);
+                tma_load_4d(smem + s * C::STAGE, &map_w, &full[s], ks * 128, 0, tile.ct * WIDTH, tile.expert, policy);
                 tc::tma_load_2d(smem + s * C::STAGE + A_BYTES, &map_x, &full[s], ks * 128, (int)tile.row0);
-                ++issued;
                 if (++s == C::STAGES) { s = 0; phase ^= 1; }
-                step(i + 1 < n);
+                step();
             }
             if (!ok) {                                                   // copies in flight land before the memory is given back
                 atomicExch(&g_w8a8_err, 1);
@@ -365,24 +405,23 @@ __global__ void __launch_bounds__(THREADS, 1) w8a8_stream_kernel(const __grid_co
             uint32_t s = 0, phase = 0, ab = 0, aphase = 0;
             const uint32_t idesc = tc::idesc_i8(NT);
             bool ok = true;
-            for (int64_t at = run.begin; at < run.end && ok;) {
-                const int k0 = (int)(at % k_steps), k1 = (int)min((int64_t)k_steps, k0 + run.end - at);
+            for (int i = 0; i < run.pieces && ok; ++i) {
+                const Piece q = piece_of(run, i);
                 if (!tc::mbar_wait(&acc_empty[ab], aphase ^ 1)) { ok = false; break; }
                 tc::tc_fence_after();
-                for (int ks = k0; ks < k1; ++ks) {
+                for (int ks = q.k0; ks < q.k1; ++ks) {
                     if (!tc::mbar_wait(&full[s], phase)) { ok = false; break; }
                     tc::tc_fence_after();
                     const uint32_t sa = tc::smem_u32(smem + s * C::STAGE), sb = sa + A_BYTES;
 #pragma unroll
                     for (int kk = 0; kk < 4; ++kk)
-                        tc::mma_i8(tmem + ab * NT, desc_sw128(sa + kk * 32), desc_sw128(sb + kk * 32), idesc, (ks - k0) | kk ? 1u : 0u);
+                        tc::mma_i8(tmem + ab * NT, desc_sw128(sa + kk * 32), desc_sw128(sb + kk * 32), idesc, (ks - q.k0) | kk ? 1u : 0u);
                     tc::mma_commit(&empty[s]);
                     if (++s == C::STAGES) { s = 0; phase ^= 1; }
                 }
                 if (!ok) break;
                 tc::mma_commit(&acc_full[ab]);
                 if (++ab == 2) { ab = 0; aphase ^= 1; }
-                at += k1 - k0;
             }
             if (!ok) atomicExch(&g_w8a8_err, 2);
             tc::mma_commit(done);
@@ -396,18 +435,18 @@ __global__ void __launch_bounds__(THREADS, 1) w8a8_stream_kernel(const __grid_co
         if (p.offsets) zero_tail<GATED>(p, row_s[p.experts], tid - 64);
         uint32_t ab = 0, aphase = 0;
         bool ok = true;                                                  // after a give-up: no more work, but every barrier of the warps
-        for (int64_t at = run.begin; at < run.end;) {
-            const int t = (int)(at / k_steps), k0 = (int)(at - (int64_t)t * k_steps), k1 = (int)min((int64_t)k_steps, k0 + run.end - at);
-            const Tile tile = order.at(t);
+        for (int i = 0; i < run.pieces; ++i) {
+            const Piece q = piece_of(run, i);
+            const Tile tile = order.at(q.t);
             float* sx = sx_s + ab * NT;
             const Lane L = make_lane<GATED>(p, tile, (int64_t)tile.ct * WIDTH, c, sx);
-            for (int i = tid - 64; i < NT; i += THREADS - 64) sx[i] = i < tile.n_rows ? p.xs[tile.row0 + i] : 0.f;
+            if (tid - 64 < NT) sx[tid - 64] = tid - 64 < tile.n_rows ? p.xs[tile.row0 + tid - 64] : 0.f;
             asm volatile("bar.sync 1, 128;" ::: "memory");               // the epilogue's own barrier
             if (ok) ok = __all_sync(0xffffffffu, tc::mbar_wait(&acc_full[ab], aphase));
             tc::tc_fence_after();
             const uint32_t base = tmem + ((uint32_t)(quarter * 32) << 16) + ab * NT;
-            const bool whole = k1 - k0 == k_steps;
-            uint32_t* slot = whole ? nullptr : p.pieces + (size_t)(2 * blockIdx.x + (k0 == 0)) * C::PIECE + c;
+            const bool whole = q.k1 - q.k0 == k_steps;
+            uint32_t* slot = whole ? nullptr : p.pieces + (size_t)(2 * blockIdx.x + (q.k0 == 0)) * C::PIECE + c;
 #pragma unroll
             for (int c0 = 0; c0 < NT; c0 += 16) {
                 uint32_t v[16];
@@ -426,7 +465,7 @@ __global__ void __launch_bounds__(THREADS, 1) w8a8_stream_kernel(const __grid_co
                 }
             }
             if (!whole) {
-                const int c_first = owner(run, (int64_t)t * k_steps), c_last = owner(run, (int64_t)t * k_steps + k_steps - 1);
+                const int c_first = owner(run, (int64_t)q.t * k_steps), c_last = owner(run, (int64_t)q.t * k_steps + k_steps - 1);
                 __threadfence();
                 asm volatile("bar.sync 1, 128;" ::: "memory");
                 if (tid == 64) {
@@ -451,7 +490,6 @@ __global__ void __launch_bounds__(THREADS, 1) w8a8_stream_kernel(const __grid_co
                 }
             }
             if (++ab == 2) { ab = 0; aphase ^= 1; }
-            at += k1 - k0;
         }
         if (!ok && lane == 0) atomicExch(&g_w8a8_err, 4);
     }
