@@ -233,8 +233,9 @@ __device__ __forceinline__ void zero_tail(const Params& p, int64_t used, int tid
 // Runs end at tile borders where that costs no more than FIXUP_STAGES stages of balance; otherwise they are of equal length,
 // and a tile cut by a border is finished by whichever of its CTAs comes last: every CTA leaves its sums in a slot of the
 // workspace and counts itself in, and the last one adds the slots (int32: in any order the same sum).  Nobody waits.
-// A CTA takes its two cut tiles first and whole tiles after them, so that the cut ones are finished while others stream
-// (4096 x 24576, 1 token: 24.3 -> ORDER_US us).
+// The usual last one is the CTA whose run ends inside the tile: the next CTA began its run with the rest of it.  It looks
+// at the count before its own sums are complete, and where all the others are in it adds their slots to its accumulator
+// and stores nothing (4096 x 24576: 24 tokens 24.9 -> 23.4 us, 64 tokens 29.1 -> 27.2 us).
 constexpr int FIXUP_STAGES = 8;
 
 struct Run {
@@ -243,7 +244,6 @@ struct Run {
     int ctas;                    // CTAs that have a run
     int k_steps;
     int pieces;                  // tiles and parts of tiles in the run
-    bool head, tail;             // begins inside a tile; ends inside another one
 };
 __device__ __forceinline__ Run make_run(const Params& p, int64_t tiles, int k_steps, int cta, int ctas)
 {
@@ -258,8 +258,6 @@ __device__ __forceinline__ Run make_run(const Params& p, int64_t tiles, int k_st
     else { r.begin = tiles * cta / ctas * k_steps; r.end = tiles * (cta + 1) / ctas * k_steps; }
     const int64_t first = r.begin / k_steps, last = (r.end + k_steps - 1) / k_steps;
     r.pieces = r.end > r.begin ? (int)(last - first) : 0;
-    r.head = r.begin % k_steps != 0;
-    r.tail = r.end % k_steps != 0 && (r.pieces > 1 || !r.head);
     return r;
 }
 // Piece i of a run: stages [k0, k1) of tile t.
@@ -268,11 +266,8 @@ struct Piece {
 };
 __device__ __forceinline__ Piece piece_of(const Run& r, int i)
 {
-    const int first = (int)(r.begin / r.k_steps), last = (int)((r.end - 1) / r.k_steps);
     Piece q;
-    if (r.head && i == 0) q.t = first;
-    else if (r.tail && i == (r.head ? 1 : 0)) q.t = last;
-    else q.t = first + i - (r.tail ? 1 : 0);
+    q.t = (int)(r.begin / r.k_steps) + i;
     const int64_t start = (int64_t)q.t * r.k_steps;
     q.k0 = (int)max((int64_t)0, r.begin - start);
     q.k1 = (int)min((int64_t)r.k_steps, r.end - start);
@@ -280,6 +275,24 @@ __device__ __forceinline__ Piece piece_of(const Run& r, int i)
 }
 // The CTA of a split whose run holds `stage`: the last one that begins at or before it.
 __device__ __forceinline__ int owner(const Run& r, int64_t stage) { return (int)(((stage + 1) * r.ctas - 1) / r.total); }
+
+__device__ __forceinline__ int ld_acquire(const int32_t* p)
+{
+    int v;
+    asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+    return v;
+}
+// Adds columns [c0, c0 + 16) of channel c from the slots of CTAs c_first..c_last but `own`.
+template <int NT>
+__device__ __forceinline__ void add_slots(const Params& p, uint32_t* v, int c0, int c, int c_first, int c_last, int own)
+{
+    for (int k = c_first; k <= c_last; ++k) {
+        if (k == own) continue;
+        const uint32_t* from = p.pieces + (size_t)(2 * k + (k == c_first)) * Stream<NT>::PIECE + c0 * 128 + c;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) v[j] += __ldcg(from + j * 128);
+    }
+}
 
 template <int NT>
 struct StreamOrder {
@@ -295,7 +308,6 @@ struct StreamOrder {
         int local = t;
         if (first) {
             while (t >= first[e + 1]) ++e;
-            while (t < first[e]) --e;
             start = row[e];
             count = row[e + 1] - row[e];
             local = t - first[e];
@@ -377,6 +389,7 @@ __global__ void __launch_bounds__(THREADS, 1) w8a8_stream_kernel(const __grid_co
                 step();
             }
             if (p.early) pdl_wait();
+            order.e = 0;
             if (n) start(0);
             for (int j = 0; j < ahead; ++j) {
                 tc::tma_load_2d(smem + j * C::STAGE + A_BYTES, &map_x, &full[j], ks * 128, (int)tile.row0);
@@ -440,13 +453,20 @@ __global__ void __launch_bounds__(THREADS, 1) w8a8_stream_kernel(const __grid_co
             const Tile tile = order.at(q.t);
             float* sx = sx_s + ab * NT;
             const Lane L = make_lane<GATED>(p, tile, (int64_t)tile.ct * WIDTH, c, sx);
+            const bool whole = q.k1 - q.k0 == k_steps;
+            int c_first = 0, c_last = 0;
+            if (!whole) {
+                c_first = owner(run, (int64_t)q.t * k_steps);
+                c_last = owner(run, (int64_t)q.t * k_steps + k_steps - 1);
+                if (tid == 64) last_s[ab] = ld_acquire(p.counters + c_first) == c_last - c_first;
+            }
             if (tid - 64 < NT) sx[tid - 64] = tid - 64 < tile.n_rows ? p.xs[tile.row0 + tid - 64] : 0.f;
             asm volatile("bar.sync 1, 128;" ::: "memory");               // the epilogue's own barrier
+            const bool last = !whole && last_s[ab];
             if (ok) ok = __all_sync(0xffffffffu, tc::mbar_wait(&acc_full[ab], aphase));
             tc::tc_fence_after();
             const uint32_t base = tmem + ((uint32_t)(quarter * 32) << 16) + ab * NT;
-            const bool whole = q.k1 - q.k0 == k_steps;
-            uint32_t* slot = whole ? nullptr : p.pieces + (size_t)(2 * blockIdx.x + (q.k0 == 0)) * C::PIECE + c;
+            uint32_t* slot = p.pieces + (size_t)(2 * blockIdx.x + (q.k0 == 0)) * C::PIECE + c;
 #pragma unroll
             for (int c0 = 0; c0 < NT; c0 += 16) {
                 uint32_t v[16];
@@ -457,15 +477,15 @@ __global__ void __launch_bounds__(THREADS, 1) w8a8_stream_kernel(const __grid_co
                     __syncwarp();
                     if (lane == 0) tc::mbar_arrive(&acc_empty[ab]);
                 }
-                if (whole) {
+                if (last && c0 < tile.n_rows) add_slots<NT>(p, v, c0, c, c_first, c_last, blockIdx.x);
+                if (whole || last) {
                     if (ok) emit<GATED, 16>(p, L, c0, v);
                 } else {
 #pragma unroll
                     for (int j = 0; j < 16; ++j) __stcg(slot + (c0 + j) * 128, v[j]);
                 }
             }
-            if (!whole) {
-                const int c_first = owner(run, (int64_t)q.t * k_steps), c_last = owner(run, (int64_t)q.t * k_steps + k_steps - 1);
+            if (!whole && !last) {
                 __threadfence();
                 asm volatile("bar.sync 1, 128;" ::: "memory");
                 if (tid == 64) {
@@ -480,11 +500,7 @@ __global__ void __launch_bounds__(THREADS, 1) w8a8_stream_kernel(const __grid_co
                         uint32_t v[16];
 #pragma unroll
                         for (int j = 0; j < 16; ++j) v[j] = 0;
-                        for (int k = c_first; k <= c_last; ++k) {
-                            const uint32_t* from = p.pieces + (size_t)(2 * k + (k == c_first)) * C::PIECE + c0 * 128 + c;
-#pragma unroll
-                            for (int j = 0; j < 16; ++j) v[j] += __ldcg(from + j * 128);
-                        }
+                        add_slots<NT>(p, v, c0, c, c_first, c_last, -1);
                         emit<GATED, 16>(p, L, c0, v);
                     }
                 }
