@@ -100,11 +100,7 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* r)
         : "memory");
 }
 // First row of expert e.  Offsets come from the caller: kept inside the rows, so that a bad one reads nothing out of range.
-__device__ __forceinline__ int64_t first_row(const Params& p, int e)
-{
-    const int32_t v = __ldcg(p.offsets + e);
-    return v < 0 ? 0 : (v < p.rows ? (int64_t)v : p.rows);
-}
+__device__ __forceinline__ int first_row(const Params& p, int e) { return max(0, min(__ldcg(p.offsets + e), (int)p.rows)); }
 
 // What a thread of the epilogue needs to turn the sums of its channel into results.
 struct Lane {
@@ -193,26 +189,50 @@ __device__ __forceinline__ Lane make_lane(const Params& p, const Tile& t, int64_
 template <typename Tiles>
 __device__ __forceinline__ void make_table(const Params& p, int32_t* first, int32_t* row, Tiles tiles_of)
 {
+    constexpr int AT_ONCE = 4;                           // 128 experts at once: latency is all that this costs
     const int lane = threadIdx.x & 31;
     int before = 0;
-    for (int e0 = 0; e0 < p.experts; e0 += 32) {
-        const int e = e0 + lane;
-        int64_t a = 0, b = 0;
-        if (e < p.experts) { a = first_row(p, e); b = first_row(p, e + 1); }
-        const int tiles = b > a ? tiles_of(b - a) * p.tiles_c : 0;
-        int scan = tiles;
+    for (int e0 = 0; e0 < p.experts; e0 += 32 * AT_ONCE) {
+        int a[AT_ONCE], b[AT_ONCE], scan[AT_ONCE], tiles[AT_ONCE];
 #pragma unroll
-        for (int d = 1; d < 32; d *= 2) {
-            const int up = __shfl_up_sync(0xffffffffu, scan, d);
-            if (lane >= d) scan += up;
+        for (int i = 0; i < AT_ONCE; ++i) {
+            const int e = e0 + 32 * i + lane;
+            a[i] = e < p.experts ? first_row(p, e) : 0;
+            b[i] = e < p.experts ? first_row(p, e + 1) : 0;
         }
-        if (e < p.experts) {
-            first[e] = before + scan - tiles;
-            row[e] = (int32_t)a;
-            if (e == p.experts - 1) { first[e + 1] = before + scan; row[e + 1] = (int32_t)b; }
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; ++i) scan[i] = tiles[i] = b[i] > a[i] ? tiles_of(b[i] - a[i]) * p.tiles_c : 0;
+#pragma unroll
+        for (int d = 1; d < 32; d *= 2)
+#pragma unroll
+            for (int i = 0; i < AT_ONCE; ++i) {
+                const int up = __shfl_up_sync(0xffffffffu, scan[i], d);
+                if (lane >= d) scan[i] += up;
+            }
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; ++i) {
+            const int e = e0 + 32 * i + lane;
+            if (e < p.experts) {
+                first[e] = before + scan[i] - tiles[i];
+                row[e] = a[i];
+                if (e == p.experts - 1) { first[e + 1] = before + scan[i]; row[e + 1] = b[i]; }
+            }
+            before += __shfl_sync(0xffffffffu, scan[i], 31);
         }
-        before += __shfl_sync(0xffffffffu, scan, 31);
     }
+}
+
+// Expert of tile t, by one full warp: the number of experts whose tiles end at or before it.
+__device__ __forceinline__ int expert_of_tile(const Params& p, const int32_t* first, int t)
+{
+    int n = 0;
+    for (int e0 = 0; e0 < p.experts; e0 += 32) {
+        const int e = e0 + (threadIdx.x & 31);
+        const uint32_t past = __ballot_sync(0xffffffffu, e < p.experts && first[e + 1] <= t);
+        n += __popc(past);
+        if (past != 0xffffffffu) break;
+    }
+    return min(n, p.experts - 1);
 }
 
 // Rows behind the last expert's become zero: dealt to the CTAs, written by the epilogue's 128 threads.
@@ -239,25 +259,27 @@ __device__ __forceinline__ void zero_tail(const Params& p, int64_t used, int tid
 constexpr int FIXUP_STAGES = 8;
 
 struct Run {
-    int64_t begin, end;          // stages of this CTA
-    int64_t total;
-    int ctas;                    // CTAs that have a run
+    int begin, end;              // stages of this CTA
+    int size, longer;            // a split: every CTA has `size` stages, the first `longer` of them one more
     int k_steps;
     int pieces;                  // tiles and parts of tiles in the run
 };
-__device__ __forceinline__ Run make_run(const Params& p, int64_t tiles, int k_steps, int cta, int ctas)
+__device__ __forceinline__ Run make_run(int tiles, int k_steps, int cta, int ctas)
 {
     Run r;
-    r.total = tiles * k_steps;
+    const int total = tiles * k_steps, per = tiles / ctas, more = tiles - per * ctas;
     r.k_steps = k_steps;
-    const int64_t whole = (tiles + ctas - 1) / ctas * k_steps, even = (r.total + ctas - 1) / ctas + FIXUP_STAGES;
-    const bool split = whole > even;
-    r.ctas = split ? (int)min((int64_t)ctas, r.total) : ctas;
-    if (cta >= r.ctas) r.begin = r.end = 0;
-    else if (split) { r.begin = r.total * cta / r.ctas; r.end = r.total * (cta + 1) / r.ctas; }
-    else { r.begin = tiles * cta / ctas * k_steps; r.end = tiles * (cta + 1) / ctas * k_steps; }
-    const int64_t first = r.begin / k_steps, last = (r.end + k_steps - 1) / k_steps;
-    r.pieces = r.end > r.begin ? (int)(last - first) : 0;
+    r.size = total / ctas;
+    r.longer = total - r.size * ctas;
+    const int whole = (per + (more ? 1 : 0)) * k_steps, even = r.size + (r.longer ? 1 : 0) + FIXUP_STAGES;
+    if (whole > even) {          // a CTA without a stage of its own (total < ctas) has an empty run
+        r.begin = cta * r.size + min(cta, r.longer);
+        r.end = r.begin + r.size + (cta < r.longer ? 1 : 0);
+    } else {
+        r.begin = (cta * per + min(cta, more)) * k_steps;
+        r.end = r.begin + (per + (cta < more ? 1 : 0)) * k_steps;
+    }
+    r.pieces = r.end > r.begin ? (r.end - 1) / k_steps - r.begin / k_steps + 1 : 0;
     return r;
 }
 // Piece i of a run: stages [k0, k1) of tile t.
@@ -267,14 +289,18 @@ struct Piece {
 __device__ __forceinline__ Piece piece_of(const Run& r, int i)
 {
     Piece q;
-    q.t = (int)(r.begin / r.k_steps) + i;
-    const int64_t start = (int64_t)q.t * r.k_steps;
-    q.k0 = (int)max((int64_t)0, r.begin - start);
-    q.k1 = (int)min((int64_t)r.k_steps, r.end - start);
+    q.t = r.begin / r.k_steps + i;
+    const int start = q.t * r.k_steps;
+    q.k0 = max(0, r.begin - start);
+    q.k1 = min(r.k_steps, r.end - start);
     return q;
 }
-// The CTA of a split whose run holds `stage`: the last one that begins at or before it.
-__device__ __forceinline__ int owner(const Run& r, int64_t stage) { return (int)(((stage + 1) * r.ctas - 1) / r.total); }
+// The CTA of a split whose run holds `stage`.
+__device__ __forceinline__ int owner(const Run& r, int stage)
+{
+    const int border = r.longer * (r.size + 1);
+    return stage < border ? stage / (r.size + 1) : r.longer + (stage - border) / r.size;
+}
 
 __device__ __forceinline__ int ld_acquire(const int32_t* p)
 {
@@ -304,20 +330,19 @@ struct StreamOrder {
     __device__ __forceinline__ Tile at(int t)
     {
         Tile r;
-        int64_t start = 0, count = p.rows;
-        int local = t;
+        int start = 0, count = (int)p.rows, local = t;
         if (first) {
             while (t >= first[e + 1]) ++e;
             start = row[e];
             count = row[e + 1] - row[e];
             local = t - first[e];
         }
-        const int tiles = (int)((count + NT - 1) / NT), tok = local % tiles;     // tokens fastest: the weights come from L2 then
-        r.ct = local / tiles;
+        const int tiles = (count + NT - 1) / NT, tok = tiles == 1 ? 0 : local % tiles;       // tokens fastest: the weights come from L2 then
+        r.ct = tiles == 1 ? local : local / tiles;
         r.nt = NT;
         r.expert = e;
-        r.row0 = start + (int64_t)tok * NT;
-        r.n_rows = (int)min((int64_t)NT, count - (int64_t)tok * NT);
+        r.row0 = start + tok * NT;
+        r.n_rows = min(NT, count - tok * NT);
         return r;
     }
 };
@@ -341,7 +366,6 @@ __global__ void __launch_bounds__(THREADS, 1) w8a8_stream_kernel(const __grid_co
     int* last_s = reinterpret_cast<int*>(tmem_slot + 1);                 // [2]
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    if (!p.early) pdl_wait();
     if (tid == 0) {
         tc::prefetch_tensormap(&map_w);
         tc::prefetch_tensormap(&map_x);
@@ -354,21 +378,23 @@ __global__ void __launch_bounds__(THREADS, 1) w8a8_stream_kernel(const __grid_co
         tc::tmem_alloc(tmem_slot, C::COLS);
         tc::tmem_relinquish();
     }
-    if (warp == 2 && p.offsets) make_table(p, first_s, row_s, [](int64_t n) { return (int)((n + NT - 1) / NT); });
+    if (!p.early) pdl_wait();
+    if (warp == 2 && p.offsets) make_table(p, first_s, row_s, [](int n) { return (n + NT - 1) / NT; });
     tc::tc_fence_before();
     __syncthreads();
     tc::tc_fence_after();
     const uint32_t tmem = *tmem_slot;
     const int k_steps = (p.K + 127) / 128;
-    const int n_tiles = p.offsets ? first_s[p.experts] : (int)((p.rows + NT - 1) / NT) * p.tiles_c;
-    const Run run = make_run(p, n_tiles, k_steps, blockIdx.x, gridDim.x);
-    StreamOrder<NT> order = {p, p.offsets ? first_s : nullptr, row_s, 0};
+    const int n_tiles = p.offsets ? first_s[p.experts] : ((int)p.rows + NT - 1) / NT * p.tiles_c;
+    const Run run = make_run(n_tiles, k_steps, blockIdx.x, gridDim.x);
+    const int e_first = p.offsets ? expert_of_tile(p, first_s, run.begin / k_steps) : 0;
+    StreamOrder<NT> order = {p, p.offsets ? first_s : nullptr, row_s, e_first};
     constexpr int WIDTH = GATED ? 64 : 128;
 
     if (warp == 0) {
         if (lane == 0) {
             const uint64_t policy = evict_first_policy();
-            const int n = (int)(run.end - run.begin);
+            const int n = run.end - run.begin;
             int i = 0, ks = 0;                                           // current piece and stage
             Piece q = {};
             Tile tile = {};
@@ -389,7 +415,7 @@ __global__ void __launch_bounds__(THREADS, 1) w8a8_stream_kernel(const __grid_co
                 step();
             }
             if (p.early) pdl_wait();
-            order.e = 0;
+            order.e = e_first;
             if (n) start(0);
             for (int j = 0; j < ahead; ++j) {
                 tc::tma_load_2d(smem + j * C::STAGE + A_BYTES, &map_x, &full[j], ks * 128, (int)tile.row0);
@@ -456,8 +482,8 @@ __global__ void __launch_bounds__(THREADS, 1) w8a8_stream_kernel(const __grid_co
             const bool whole = q.k1 - q.k0 == k_steps;
             int c_first = 0, c_last = 0;
             if (!whole) {
-                c_first = owner(run, (int64_t)q.t * k_steps);
-                c_last = owner(run, (int64_t)q.t * k_steps + k_steps - 1);
+                c_first = owner(run, q.t * k_steps);
+                c_last = owner(run, q.t * k_steps + k_steps - 1);
                 if (tid == 64) last_s[ab] = ld_acquire(p.counters + c_first) == c_last - c_first;
             }
             if (tid - 64 < NT) sx[tid - 64] = tid - 64 < tile.n_rows ? p.xs[tile.row0 + tid - 64] : 0.f;
@@ -616,14 +642,14 @@ w8a8_pair_kernel(const __grid_constant__ PairMaps maps, const Params p, int band
         tc::tmem_alloc_pair(tmem_slot, 512);
         tc::tmem_relinquish_pair();
     }
-    if (warp == 0 && p.offsets) make_table(p, first_s, row_s, [](int64_t n) { return token_tiles(n); });
+    if (warp == 0 && p.offsets) make_table(p, first_s, row_s, [](int n) { return token_tiles(n); });
     tc::tc_fence_before();
     __syncthreads();
     tc::cluster_sync_all();                              // the other CTA's barriers exist before anything targets them
     tc::tc_fence_after();
     const uint32_t tmem = *tmem_slot;
     const int n_tiles = p.offsets ? first_s[p.experts] : token_tiles(p.rows) * p.tiles_c;
-    TileOrder order = {p, p.offsets ? first_s : nullptr, row_s, band, 0};
+    TileOrder order = {p, p.offsets ? first_s : nullptr, row_s, band, p.offsets ? expert_of_tile(p, first_s, pair) : 0};
     const int k_steps = (p.K + 127) / 128;
     constexpr int WIDTH = GATED ? 64 : 128;              // channels of the result per CTA
 
@@ -1043,9 +1069,10 @@ WUSH_API int wush_w8a8_linear(const void* x, int dtype, const int8_t* wq, const 
 }
 
 // ---- the expert block ----------------------------------------------------------------------------------------------------
-// sort -> gather + quantise -> gated product -> quantise -> product -> weighted sum, six launches, each but the first allowed
-// to start under the one before it.  Every kernel of the chain first waits for the one in front and only then lets the next
-// one start, so what was written two launches earlier is there without a wait.
+// sort -> gather + quantise -> gated product -> quantise -> product -> weighted sum, each but
+// the first launch allowed to start under the one before it.  What a kernel reads before its wait is older than the kernel
+// in front of it: a kernel lets the next one start only after its own wait, but for the second quantiser, whose successor
+// reads nothing before its wait that was not there when the quantiser started.
 namespace {
 struct FfnPlan {
     int64_t R;
@@ -1107,10 +1134,10 @@ WUSH_API int wush_w8a8_expert_ffn(const void* x, int dtype, const void* ids, int
     if (int e = check_product("w8a8_expert_ffn", down)) return e;
     if (int e = ensure_init()) return e;
     cudaStream_t st = (cudaStream_t)stream;
-    if (int e = expert_sort_launch(ids, id_bytes, f.R, (int)experts, pos, offsets, st)) return e;
     const bool counted = w8a8_workspace_bytes(f.R, experts) != 0;       // both products of a block run on the same kernel
     const QuantRows qx = {x, dtype, tokens, H, xq, xs, pos, (int)k, offsets + experts, counted ? (int32_t*)(base + f.up) : nullptr};
     const QuantRows qh = {h, WUSH_F32, f.R, I, hq, hs, nullptr, 1, nullptr, counted ? (int32_t*)(base + f.down) : nullptr};
+    if (int e = expert_sort_launch(ids, id_bytes, f.R, (int)experts, pos, offsets, st)) return e;
     if (int e = quant_int8_launch(qx, true, st)) return e;
     if (int e = w8a8_launch(up, base + f.up, true, st)) return e;
     if (int e = quant_int8_launch(qh, true, st)) return e;

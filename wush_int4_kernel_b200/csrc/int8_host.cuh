@@ -22,7 +22,7 @@ static inline int check_entries(const char* op, int64_t tokens, int64_t k, int64
 
 // Launchers used by the entry points of one operator and by the expert block, which chains them.  `dependent`: launched
 // with programmatic serialisation, so the kernel may start under the one before it; it waits for that one before it reads
-// anything that a kernel wrote.
+// anything that the one before it wrote.
 struct QuantRows {
     const void* x;
     int dtype;
@@ -54,6 +54,7 @@ struct W8A8Problem {
 // The product's workspace: counters, which are zero when its kernel starts, then slots.
 constexpr size_t W8A8_COUNTER_BYTES = 1024;
 size_t w8a8_workspace_bytes(int64_t rows, int64_t experts);
+// Dependent: weights and offsets are older than the kernel in front, so they are read before the wait for it.
 int w8a8_launch(const W8A8Problem& p, void* workspace, bool dependent, cudaStream_t st);
 
 }  // namespace wush

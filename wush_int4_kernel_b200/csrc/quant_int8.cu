@@ -113,93 +113,131 @@ __device__ __forceinline__ uint4 codes16(const Raw16<T>& r, float inv, bool tiny
     return make_uint4(o[0], o[1], o[2], o[3]);
 }
 
-// One row per group of `tpr` threads (a power of two, 32 .. blockDim.x).
+// A row of K elements in the hands of `tpr` threads (a power of two, 32 .. blockDim.x); `lane`: this thread among them.
+template <typename T>
+struct Row {
+    const T* x;
+    int vecs, lane, tpr;
+    Raw16<T> held[HOLD];
+    float scale, inv;
+    bool tiny;
+
+    // Largest magnitude over the row, then its scale.  Every thread of the block takes part; `part`: 32 words of shared memory.
+    __device__ __forceinline__ void find_scale(bool live, uint32_t* part)
+    {
+        uint32_t m = 0;
+        if (live) {
+#pragma unroll
+            for (int i = 0; i < HOLD; ++i)
+                if (lane + i * tpr < vecs) held[i] = load16<T>(x + (int64_t)(lane + i * tpr) * VEC);
+#pragma unroll
+            for (int i = 0; i < HOLD; ++i)
+                if (lane + i * tpr < vecs) m = amax_bits<T>(held[i], m);
+            for (int v = lane + HOLD * tpr; v < vecs; v += tpr) m = amax_bits<T>(load16<T>(x + (int64_t)v * VEC), m);
+        }
+        if constexpr (sizeof(T) == 2) m = max(m & 0xffffu, m >> 16);
+        m = __reduce_max_sync(0xffffffffu, m);
+        if (tpr > 32) {                                         // the same choice in the whole block
+            if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = m;
+            __syncthreads();
+            const int w0 = threadIdx.x / tpr * (tpr >> 5);
+            m = part[w0 + ((threadIdx.x & 31) & ((tpr >> 5) - 1))];
+            m = __reduce_max_sync(0xffffffffu, m);
+        }
+        const float amax = value_of_bits<T>(m);
+        const bool finite = amax < __int_as_float(0x7f800000);
+        tiny = amax < 0x1p-100f;
+        inv = finite && amax > 0.f ? __fdiv_rn(127.f, tiny ? amax * 0x1p100f : amax) : 0.f;
+        scale = finite ? __fdiv_rn(amax, 127.f) : amax;
+    }
+    // Calls put(step, codes) for every 16 elements of this thread.
+    template <typename F>
+    __device__ __forceinline__ void codes(F put) const
+    {
+        const uint4 zero = make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < HOLD; ++i)
+            if (lane + i * tpr < vecs) put(lane + i * tpr, inv > 0.f ? codes16<T>(held[i], inv, tiny) : zero);
+        for (int v = lane + HOLD * tpr; v < vecs; v += tpr)
+            put(v, inv > 0.f ? codes16<T>(load16<T>(x + (int64_t)v * VEC), inv, tiny) : zero);
+    }
+    // Codes and scale to row r, or to the rows of k entries (those outside [0, total) are no rows).
+    __device__ __forceinline__ void store(int8_t* q, float* s, int64_t r) const
+    {
+        codes([&](int v, const uint4& c) { *reinterpret_cast<uint4*>(q + (r * vecs + v) * VEC) = c; });
+        if (lane == 0) s[r] = scale;
+    }
+    __device__ __forceinline__ void store(int8_t* q, float* s, const int32_t* pos, int k, int64_t total) const
+    {
+        codes([&](int v, const uint4& c) {
+            for (int j = 0; j < k; ++j) {
+                const int64_t r = pos[j];
+                if (r >= 0 && r < total) *reinterpret_cast<uint4*>(q + (r * vecs + v) * VEC) = c;
+            }
+        });
+        for (int j = lane; j < k; j += tpr) {
+            const int64_t r = pos[j];
+            if (r >= 0 && r < total) s[r] = scale;
+        }
+    }
+};
+
+// Rows behind the last entry of an expert become zero, dealt to the blocks.
+__device__ __forceinline__ void zero_tail(int8_t* q, float* s, int vecs, int64_t used, int64_t total)
+{
+    for (int64_t r = (used > 0 ? used : 0) + blockIdx.x; r < total; r += gridDim.x) {
+        for (int v = threadIdx.x; v < vecs; v += blockDim.x) *reinterpret_cast<uint4*>(q + (r * vecs + v) * VEC) = make_uint4(0, 0, 0, 0);
+        if (threadIdx.x == 0) s[r] = 0.f;
+    }
+}
+__device__ __forceinline__ void zero_counters(int32_t* counters)
+{
+    if (counters && blockIdx.x == 0)
+        for (int i = threadIdx.x; i < (int)(W8A8_COUNTER_BYTES / 4); i += blockDim.x) counters[i] = 0;
+}
+
 template <typename T>
 __global__ void __launch_bounds__(1024) quant_int8_kernel(const T* __restrict__ x, int64_t rows, int K, int tpr,
                                                           int8_t* __restrict__ q, float* __restrict__ s,
                                                           const int32_t* __restrict__ pos, int k,
                                                           const int32_t* __restrict__ n_used, int32_t* __restrict__ counters)
 {
-    pdl_wait();
-    pdl_launch_dependents();
     __shared__ uint32_t part[32];
-    if (counters && blockIdx.x == 0)
-        for (int i = threadIdx.x; i < (int)(W8A8_COUNTER_BYTES / 4); i += blockDim.x) counters[i] = 0;
-    const int group = threadIdx.x / tpr, lane = threadIdx.x - group * tpr;
-    const int64_t row = (int64_t)blockIdx.x * (blockDim.x / tpr) + group;
-    const int vecs = K / VEC;
-    const bool live = row < rows;
-    const T* xr = x + row * K;
-    Raw16<T> held[HOLD];
-    uint32_t m = 0;
-    if (live) {
-#pragma unroll
-        for (int i = 0; i < HOLD; ++i)
-            if (lane + i * tpr < vecs) held[i] = load16<T>(xr + (int64_t)(lane + i * tpr) * VEC);
-#pragma unroll
-        for (int i = 0; i < HOLD; ++i)
-            if (lane + i * tpr < vecs) m = amax_bits<T>(held[i], m);
-        for (int v = lane + HOLD * tpr; v < vecs; v += tpr) m = amax_bits<T>(load16<T>(xr + (int64_t)v * VEC), m);
+    // In front of a gather runs the sort, which writes positions but not the rows to be quantised: those are read at once.
+    // Behind a gated product, the product that follows may start at once: before its own wait it reads weights and offsets,
+    // which were there before this kernel started.
+    if (!pos) {
+        pdl_launch_dependents();
+        pdl_wait();
     }
-    if constexpr (sizeof(T) == 2) m = max(m & 0xffffu, m >> 16);
-    m = __reduce_max_sync(0xffffffffu, m);
-    if (tpr > 32) {                                             // the same choice in the whole block
-        if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = m;
-        __syncthreads();
-        const int w0 = group * (tpr >> 5);
-        m = part[w0 + ((threadIdx.x & 31) & ((tpr >> 5) - 1))];
-        m = __reduce_max_sync(0xffffffffu, m);
+    const int64_t row = (int64_t)blockIdx.x * (blockDim.x / tpr) + threadIdx.x / tpr;
+    Row<T> r = {x + row * K, K / VEC, (int)threadIdx.x & (tpr - 1), tpr};
+    r.find_scale(row < rows, part);
+    if (pos) {
+        pdl_wait();
+        pdl_launch_dependents();
     }
-    if (live) {
-        const float amax = value_of_bits<T>(m);
-        const bool finite = amax < __int_as_float(0x7f800000);
-        const bool tiny = amax < 0x1p-100f;
-        const bool used = finite && amax > 0.f;
-        const float inv = used ? __fdiv_rn(127.f, tiny ? amax * 0x1p100f : amax) : 0.f;
-        const float scale = finite ? __fdiv_rn(amax, 127.f) : amax;
-        auto put = [&](int v, const Raw16<T>& raw) {
-            uint4 c = make_uint4(0, 0, 0, 0);
-            if (used) c = codes16<T>(raw, inv, tiny);
-            if (!pos) {
-                *reinterpret_cast<uint4*>(q + row * K + (int64_t)v * VEC) = c;
-            } else {
-                for (int j = 0; j < k; ++j) {
-                    const int64_t p = pos[row * k + j];
-                    if (p >= 0 && p < rows * k) *reinterpret_cast<uint4*>(q + p * K + (int64_t)v * VEC) = c;
-                }
-            }
-        };
-#pragma unroll
-        for (int i = 0; i < HOLD; ++i)
-            if (lane + i * tpr < vecs) put(lane + i * tpr, held[i]);
-        for (int v = lane + HOLD * tpr; v < vecs; v += tpr) put(v, load16<T>(xr + (int64_t)v * VEC));
-        if (!pos) {
-            if (lane == 0) s[row] = scale;
-        } else {
-            for (int j = lane; j < k; j += tpr) {
-                const int64_t p = pos[row * k + j];
-                if (p >= 0 && p < rows * k) s[p] = scale;
-            }
-        }
+    zero_counters(counters);
+    if (row < rows) {
+        if (pos) r.store(q, s, pos + row * k, k, rows * k);
+        else r.store(q, s, row);
     }
-    if (n_used) {                                               // rows behind the last entry of an expert: zero
-        const int64_t total = rows * k;
-        for (int64_t r = (int64_t)max(*n_used, 0) + blockIdx.x; r < total; r += gridDim.x) {
-            for (int v = threadIdx.x; v < vecs; v += blockDim.x)
-                *reinterpret_cast<uint4*>(q + r * K + (int64_t)v * VEC) = make_uint4(0, 0, 0, 0);
-            if (threadIdx.x == 0) s[r] = 0.f;
-        }
-    }
+    if (n_used) zero_tail(q, s, K / VEC, *n_used, rows * k);
+}
+
+// Threads per row.  Few rows: a thread for every 16 elements.  Many: two steps per thread, which the registers hold.
+int threads_per_row(int64_t rows, int64_t K)
+{
+    const int vecs = (int)(K / VEC), want = rows <= 2 * sm_count() ? vecs : (vecs + HOLD - 1) / HOLD;
+    int tpr = 32;
+    while (tpr < want && tpr < 1024) tpr *= 2;
+    return tpr;
 }
 
 template <typename T>
 int launch_quant(const QuantRows& a, bool dependent, cudaStream_t st)
 {
-    const int vecs = (int)(a.K / VEC);
-    // Few rows: a thread for every 16 elements.  Many: two steps per thread, which the registers hold.
-    const int want = a.rows <= 2 * sm_count() ? vecs : (vecs + HOLD - 1) / HOLD;
-    int tpr = 32;
-    while (tpr < want && tpr < 1024) tpr *= 2;
+    const int tpr = threads_per_row(a.rows, a.K);
     const int block = tpr < 256 ? 256 : tpr;
     const int64_t per = block / tpr, grid = (a.rows + per - 1) / per;
     if (grid > 0x7fffffffll) return fail(WUSH_ERR_UNSUPPORTED, "quant_int8: too many rows (%lld)", (long long)a.rows);
