@@ -111,42 +111,57 @@ struct Lane {
     const float* sx;             // token scales in shared memory
 };
 
-// Results of COUNT tokens from m0 (even) on.  The two lanes of a pair exchange one value for every two tokens m, m + 1: the
-// even lane ends with both values of token m, the odd lane with both of token m + 1, so that 16-bit results leave as 4-byte
-// stores (64 bytes per token and warp) and a gated pair meets without another exchange.  Straight-line code: a branch per
-// pair left the warp waiting for one shuffle after another (14 us per 128 x 256 tile, 4 with this).
+// Results of COUNT tokens from m0 (a multiple of four) on.  The two lanes of a pair exchange one value for every two tokens m,
+// m + 1: the even lane ends with both values of token m, the odd lane with both of token m + 1, so that 16-bit results leave
+// as 4-byte stores (64 bytes per token and warp) and a gated pair meets without another exchange.  Straight-line code, and
+// scales loaded before the first store: with a branch per pair, or with loads that wait for the stores in front of them
+// because they might alias, a warp stalls once per pair (gated, 32 tokens: 1.7 us; as it stands EMIT_US).
 template <bool GATED, int COUNT>
 __device__ __forceinline__ void emit(const Params& p, const Lane& L, int m0, const uint32_t* v)
 {
     const int odd = threadIdx.x & 1;
     const int left = L.n_rows - m0;                      // tokens that exist
     if (left <= 0) return;
-    auto scaled = [&](int j) { return __fmul_rn((float)(int)v[j], __fmul_rn(L.sx[m0 + j], L.sw)); };
+    float f[COUNT];
+#pragma unroll
+    for (int j = 0; j < COUNT; j += 4) {
+        const float4 sx = *reinterpret_cast<const float4*>(L.sx + m0 + j);
+        f[j] = __fmul_rn((float)(int)v[j], __fmul_rn(sx.x, L.sw));
+        f[j + 1] = __fmul_rn((float)(int)v[j + 1], __fmul_rn(sx.y, L.sw));
+        f[j + 2] = __fmul_rn((float)(int)v[j + 2], __fmul_rn(sx.z, L.sw));
+        f[j + 3] = __fmul_rn((float)(int)v[j + 3], __fmul_rn(sx.w, L.sw));
+    }
     if constexpr (GATED) {
+        float h[COUNT / 2];
+#pragma unroll
+        for (int j = 0; j < COUNT; j += 2) {
+            const float got = __shfl_xor_sync(0xffffffffu, odd ? f[j] : f[j + 1], 1);
+            const float g = odd ? got : f[j], u = odd ? f[j + 1] : got;
+            h[j / 2] = __fmul_rn(__fdividef(g, 1.f + expf(-g)), u);
+        }
         float* y = reinterpret_cast<float*>(p.y) + (L.row0 + m0 + odd) * p.N + L.n;
         const bool mine = L.n < p.N;
 #pragma unroll
         for (int j = 0; j < COUNT; j += 2) {
-            const float f0 = scaled(j), f1 = scaled(j + 1);
-            const float got = __shfl_xor_sync(0xffffffffu, odd ? f0 : f1, 1);
-            const float g = odd ? got : f0, u = odd ? f1 : got;
-            const float h = __fmul_rn(__fdividef(g, 1.f + expf(-g)), u);
-            if (mine && j + odd < left) *y = h;
+            if (mine && j + odd < left) *y = h[j / 2];
             y += 2 * p.N;
         }
     } else if ((p.N & 1) == 0) {
         const int64_t n = L.n & ~int64_t(1);
+        uint32_t w[COUNT / 2];
+#pragma unroll
+        for (int j = 0; j < COUNT; j += 2) {
+            const float f0 = __fadd_rn(f[j], L.bias), f1 = __fadd_rn(f[j + 1], L.bias);
+            const float got = __shfl_xor_sync(0xffffffffu, odd ? f0 : f1, 1);
+            const float lo = odd ? got : f0, hi = odd ? f1 : got;
+            if (p.bf16_out) { __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi); w[j / 2] = *reinterpret_cast<uint32_t*>(&h); }
+            else { __half2 h = __floats2half2_rn(lo, hi); w[j / 2] = *reinterpret_cast<uint32_t*>(&h); }
+        }
         uint32_t* y = reinterpret_cast<uint32_t*>(reinterpret_cast<uint16_t*>(p.y) + (L.row0 + m0 + odd) * p.N + n);
         const bool mine = n < p.N;
 #pragma unroll
         for (int j = 0; j < COUNT; j += 2) {
-            const float f0 = __fadd_rn(scaled(j), L.bias), f1 = __fadd_rn(scaled(j + 1), L.bias);
-            const float got = __shfl_xor_sync(0xffffffffu, odd ? f0 : f1, 1);
-            const float lo = odd ? got : f0, hi = odd ? f1 : got;
-            uint32_t w;
-            if (p.bf16_out) { __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi); w = *reinterpret_cast<uint32_t*>(&h); }
-            else { __half2 h = __floats2half2_rn(lo, hi); w = *reinterpret_cast<uint32_t*>(&h); }
-            if (mine && j + odd < left) *y = w;
+            if (mine && j + odd < left) *y = w[j / 2];
             y += p.N;
         }
     } else {                                             // rows of an odd number of channels: 2-byte stores
@@ -154,8 +169,8 @@ __device__ __forceinline__ void emit(const Params& p, const Lane& L, int m0, con
         const bool mine = L.n < p.N;
 #pragma unroll
         for (int j = 0; j < COUNT; ++j) {
-            const float f = __fadd_rn(scaled(j), L.bias);
-            const uint16_t w = p.bf16_out ? __bfloat16_as_ushort(__float2bfloat16_rn(f)) : __half_as_ushort(__float2half_rn(f));
+            const float r = __fadd_rn(f[j], L.bias);
+            const uint16_t w = p.bf16_out ? __bfloat16_as_ushort(__float2bfloat16_rn(r)) : __half_as_ushort(__float2half_rn(r));
             if (mine && j < left) *y = w;
             y += p.N;
         }
