@@ -250,12 +250,12 @@ __device__ __forceinline__ int expert_of_tile(const Params& p, const int32_t* fi
     return min(n, p.experts - 1);
 }
 
-// Rows behind the last expert's become zero: dealt to the CTAs, written by the epilogue's 128 threads.
+// Rows behind the last expert's become zero: dealt to the CTAs, written by the epilogue's threads.
 template <bool GATED>
-__device__ __forceinline__ void zero_tail(const Params& p, int64_t used, int tid)
+__device__ __forceinline__ void zero_tail(const Params& p, int64_t used, int tid, int threads)
 {
     for (int64_t r = used + blockIdx.x; r < p.rows; r += gridDim.x)
-        for (int64_t i = tid; i < p.N; i += 128) {
+        for (int64_t i = tid; i < p.N; i += threads) {
             if constexpr (GATED) reinterpret_cast<float*>(p.y)[r * p.N + i] = 0.f;
             else reinterpret_cast<uint16_t*>(p.y)[r * p.N + i] = 0;
         }
@@ -486,7 +486,7 @@ __global__ void __launch_bounds__(THREADS, 1) w8a8_stream_kernel(const __grid_co
         if (p.early) pdl_wait();
         pdl_launch_dependents();
         const int quarter = warp & 3, c = quarter * 32 + lane;           // tcgen05.ld: a warp reads lanes 32 * (warp % 4) ...
-        if (p.offsets) zero_tail<GATED>(p, row_s[p.experts], tid - 64);
+        if (p.offsets) zero_tail<GATED>(p, row_s[p.experts], tid - 64, 128);
         uint32_t ab = 0, aphase = 0;
         bool ok = true;                                                  // after a give-up: no more work, but every barrier of the warps
         for (int i = 0; i < run.pieces; ++i) {
@@ -561,6 +561,7 @@ __global__ void __launch_bounds__(THREADS, 1) w8a8_stream_kernel(const __grid_co
 // pairs are persistent.  The token count of a tile is a multiple of 32 chosen per expert (its rows in equal tiles), so a
 // ragged expert costs MMAs for at most 31 rows that do not exist, not for a full tile.
 constexpr int PAIR_TOKENS = 256, PAIR_STAGES = 6, PAIR_ACC = 2;
+constexpr int PAIR_EPILOGUE = 256, PAIR_THREADS = 64 + PAIR_EPILOGUE;     // eight epilogue warps: two share a quarter of the lanes
 constexpr int PAIR_STAGE = 2 * A_BYTES;                  // 128 weight rows and up to 128 token rows
 constexpr int PAIR_SX = PAIR_STAGES * PAIR_STAGE;        // token scales of two tiles
 constexpr int PAIR_TABLE = PAIR_SX + 2 * PAIR_TOKENS * 4;
@@ -584,8 +585,8 @@ __device__ __forceinline__ void tma_load_4d_pair(void* dst, const CUtensorMap* m
 }
 
 // Token tiles of `count` rows: as few as possible, of equal size.  (tiles - 1) * nt < count, because nt <= 256.
-__host__ __device__ __forceinline__ int token_tiles(int64_t count) { return (int)((count + PAIR_TOKENS - 1) / PAIR_TOKENS); }
-__device__ __forceinline__ int tile_width(int64_t count, int tiles) { return (int)(((count + tiles - 1) / tiles + 31) & ~31ll); }
+__host__ __device__ __forceinline__ int token_tiles(int count) { return (int)(((unsigned)count + PAIR_TOKENS - 1) / PAIR_TOKENS); }
+__device__ __forceinline__ int tile_width(int count, int tiles) { return tiles == 1 ? (count + 31) & ~31 : (int)((((unsigned)count + tiles - 1) / (unsigned)tiles + 31) & ~31u); }
 
 // Tile t in the order in which the pairs take them.  Inside a group of token tiles the tokens run fastest, so tiles that
 // run together share weight rows and one wave's weights are read from HBM once.  Groups: the experts, or, with one
@@ -599,34 +600,35 @@ struct TileOrder {
     __device__ __forceinline__ Tile at(int t)
     {
         Tile r;
-        int64_t count, start;
-        int tok;
+        int count, start, tok, local = t, here;
         if (first) {
             while (t >= first[e + 1]) ++e;
             start = row[e];
-            count = row[e + 1] - row[e];
-            const int tiles = token_tiles(count), local = t - first[e];
-            tok = local % tiles;
-            r.ct = local / tiles;
-            r.nt = tile_width(count, tiles);
+            count = row[e + 1] - start;
+            local = t - first[e];
+            here = token_tiles(count);
+            r.nt = tile_width(count, here);
+            tok = 0;
         } else {
             start = 0;
-            count = p.rows;
-            const int tiles = token_tiles(count), b = t / (band * p.tiles_c), local = t - b * band * p.tiles_c;
-            const int here = min(band, tiles - b * band);
-            tok = b * band + local % here;
-            r.ct = local / here;
+            count = (int)p.rows;
+            const int tiles = token_tiles(count), b = band >= tiles ? 0 : t / (band * p.tiles_c);
+            local = t - b * band * p.tiles_c;
+            here = min(band, tiles - b * band);
             r.nt = tile_width(count, tiles);
+            tok = b * band;
         }
+        r.ct = here == 1 ? local : (int)((unsigned)local / (unsigned)here);
+        tok += local - r.ct * here;
         r.expert = e;
-        r.row0 = start + (int64_t)tok * r.nt;
-        r.n_rows = (int)min((int64_t)r.nt, count - (int64_t)tok * r.nt);
+        r.row0 = (int64_t)start + tok * r.nt;
+        r.n_rows = min(r.nt, count - tok * r.nt);
         return r;
     }
 };
 
 template <bool GATED>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
 w8a8_pair_kernel(const __grid_constant__ PairMaps maps, const Params p, int band)
 {
     extern __shared__ uint8_t smem_raw[];
@@ -649,7 +651,7 @@ w8a8_pair_kernel(const __grid_constant__ PairMaps maps, const Params p, int band
     pdl_launch_dependents();
     if (tid == 0) {
         for (int i = 0; i < PAIR_STAGES; ++i) { tc::mbar_init(&full[i], 1); tc::mbar_init(&empty[i], 1); }
-        for (int i = 0; i < PAIR_ACC; ++i) { tc::mbar_init(&acc_full[i], 1); tc::mbar_init(&acc_empty[i], 8); }
+        for (int i = 0; i < PAIR_ACC; ++i) { tc::mbar_init(&acc_full[i], 1); tc::mbar_init(&acc_empty[i], 2 * PAIR_EPILOGUE / 32); }
         tc::mbar_init(done_bar, 1);
         tc::mbar_fence_init();
     }
@@ -663,7 +665,7 @@ w8a8_pair_kernel(const __grid_constant__ PairMaps maps, const Params p, int band
     tc::cluster_sync_all();                              // the other CTA's barriers exist before anything targets them
     tc::tc_fence_after();
     const uint32_t tmem = *tmem_slot;
-    const int n_tiles = p.offsets ? first_s[p.experts] : token_tiles(p.rows) * p.tiles_c;
+    const int n_tiles = p.offsets ? first_s[p.experts] : token_tiles((int)p.rows) * p.tiles_c;
     TileOrder order = {p, p.offsets ? first_s : nullptr, row_s, band, p.offsets ? expert_of_tile(p, first_s, pair) : 0};
     const int k_steps = (p.K + 127) / 128;
     constexpr int WIDTH = GATED ? 64 : 128;              // channels of the result per CTA
@@ -707,9 +709,8 @@ w8a8_pair_kernel(const __grid_constant__ PairMaps maps, const Params p, int band
         if (lane == 0 && rank == 0) {
             uint32_t slot = 0, phase = 0, ab = 0, aphase = 0;
             bool ok = true;
+            uint32_t idesc = pair < n_tiles ? tc::idesc_i8_pair(order.at(pair).nt) : 0, next = 0;
             for (int t = pair; t < n_tiles && ok; t += n_pairs) {
-                const Tile tile = order.at(t);
-                const uint32_t idesc = tc::idesc_i8_pair(tile.nt);
                 if (!tc::mbar_wait(&acc_empty[ab], aphase ^ 1)) { ok = false; break; }
                 tc::tc_fence_after();
                 for (int ks = 0; ks < k_steps; ++ks) {
@@ -721,7 +722,10 @@ w8a8_pair_kernel(const __grid_constant__ PairMaps maps, const Params p, int band
                         tc::mma_i8_pair(tmem + ab * PAIR_TOKENS, desc_sw128(sa + kk * 32), desc_sw128(sb + kk * 32), idesc, (ks | kk) ? 1u : 0u);
                     tc::mma_commit_pair(&empty[slot]);                           // frees the stage in both CTAs
                     if (++slot == PAIR_STAGES) { slot = 0; phase ^= 1; }
+                    // The next tile's width, while the tensor core has stages to work on: between two tiles it would wait for it.
+                    if (ks == (k_steps > 2 ? 2 : 0) && t + n_pairs < n_tiles) next = tc::idesc_i8_pair(order.at(t + n_pairs).nt);
                 }
+                idesc = next;
                 if (!ok) break;
                 tc::mma_commit_pair(&acc_full[ab]);                              // both CTAs' epilogues may read
                 if (++ab == PAIR_ACC) { ab = 0; aphase ^= 1; }
@@ -734,30 +738,42 @@ w8a8_pair_kernel(const __grid_constant__ PairMaps maps, const Params p, int band
     } else {
         const int quarter = warp & 3, c = quarter * 32 + lane;                   // tcgen05.ld: a warp reads lanes 32 * (warp % 4) ...
         const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
-        if (p.offsets) zero_tail<GATED>(p, row_s[p.experts], tid - 64);
+        if (p.offsets) zero_tail<GATED>(p, row_s[p.experts], tid - 64, PAIR_EPILOGUE);
+        const int half = (warp - 2) >> 2, me = tid - 64;                         // the two warps of a quarter take every other chunk
         uint32_t ab = 0, aphase = 0;
-        bool ok = true;
+        bool ok = true;                                                          // after a give-up: no more work, but every barrier of the warps
+        Tile tile = {};
+        Lane L = {};
+        float sx_mine = 0.f;                                                     // scale of token `me` of the tile
+        auto fetch = [&](int t) {
+            tile = order.at(t);
+            L = make_lane<GATED>(p, tile, (int64_t)tile.ct * 2 * WIDTH + rank * WIDTH, c, nullptr);
+            sx_mine = me < tile.n_rows ? p.xs[tile.row0 + me] : 0.f;
+        };
+        if (pair < n_tiles) fetch(pair);
         for (int t = pair; t < n_tiles; t += n_pairs) {
-            const Tile tile = order.at(t);
             float* sx = sx_s + ab * PAIR_TOKENS;
-            const Lane L = make_lane<GATED>(p, tile, (int64_t)tile.ct * 2 * WIDTH + rank * WIDTH, c, sx);
-            for (int i = tid - 64; i < tile.nt; i += THREADS - 64) sx[i] = i < tile.n_rows ? p.xs[tile.row0 + i] : 0.f;
-            asm volatile("bar.sync 1, 128;" ::: "memory");                       // the epilogue's own barrier
+            if (me < tile.nt) sx[me] = sx_mine;
+            asm volatile("bar.sync 1, 256;" ::: "memory");                       // the epilogue's own barrier
+            Lane now = L;
+            now.sx = sx;
+            const int chunks = tile.nt / 32;
+            if (t + n_pairs < n_tiles) fetch(t + n_pairs);                       // the next tile's scales arrive under this one's work
             if (ok) ok = __all_sync(0xffffffffu, tc::mbar_wait(&acc_full[ab], aphase));
             tc::tc_fence_after();
-            const int chunks = ok ? tile.nt / 32 : 0;                            // after a give-up: no more work, but every barrier of the warps
 #pragma unroll 1
-            for (int c0 = 0; c0 < chunks; ++c0) {
+            for (int c0 = half; c0 < chunks && ok; c0 += 2) {
                 uint32_t v[32];
                 tc::tmem_ld32(tmem + lane_base + ab * PAIR_TOKENS + c0 * 32, v);
                 tc::tmem_ld_wait();
-                if (c0 == chunks - 1) {
+                if (c0 + 2 >= chunks) {
                     tc::tc_fence_before();
                     __syncwarp();
                     if (lane == 0) tc::mbar_arrive_cluster(tc::map_to_rank(&acc_empty[ab], 0));
                 }
-                emit<GATED, 32>(p, L, c0 * 32, v);
+                emit<GATED, 32>(p, now, c0 * 32, v);
             }
+            if (half >= chunks && lane == 0) tc::mbar_arrive_cluster(tc::map_to_rank(&acc_empty[ab], 0));
             if (++ab == PAIR_ACC) { ab = 0; aphase ^= 1; }
         }
         if (!ok && lane == 0) atomicExch(&g_w8a8_err, 4);
@@ -855,14 +871,14 @@ int launch_pair(const W8A8Problem& w, Params p, bool dependent, cudaStream_t st)
     int dev = 0;
     cudaGetDevice(&dev);
     const int resident = dev >= 0 && dev < 64 && g_pairs_resident[dev] > 0 ? g_pairs_resident[dev] : sm_count() / 2;
-    const int64_t most = ((int64_t)token_tiles(w.rows) + (w.offsets ? std::min(w.experts, w.rows) : 0)) * p.tiles_c;
+    const int64_t most = ((int64_t)token_tiles((int)w.rows) + (w.offsets ? std::min(w.experts, w.rows) : 0)) * p.tiles_c;
     if (most > 0x7fffffffll) return fail(WUSH_ERR_UNSUPPORTED, "w8a8: too many tiles (%lld)", (long long)most);
     const int pairs = (int)std::min<int64_t>(most, resident);
     // Band of token tiles whose activations take about a quarter of the L2 (32 MB).
-    const int band = (int)std::max<int64_t>(2, std::min<int64_t>(token_tiles(w.rows), (32ll << 20) / (PAIR_TOKENS * w.K)));
+    const int band = (int)std::max<int64_t>(2, std::min<int64_t>(token_tiles((int)w.rows), (32ll << 20) / (PAIR_TOKENS * w.K)));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(2 * pairs);
-    cfg.blockDim = dim3(THREADS);
+    cfg.blockDim = dim3(PAIR_THREADS);
     cfg.dynamicSmemBytes = PAIR_SMEM;
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
@@ -885,7 +901,7 @@ int set_pair()
     if (dev < 0 || dev >= 64) return WUSH_OK;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(sm_count() & ~1));
-    cfg.blockDim = dim3(THREADS);
+    cfg.blockDim = dim3(PAIR_THREADS);
     cfg.dynamicSmemBytes = PAIR_SMEM;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
