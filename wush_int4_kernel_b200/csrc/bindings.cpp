@@ -4,6 +4,7 @@
 // outputs (and scratch) through torch's caching allocator, pick the current stream and
 // launch -- no host synchronisation, so every op can be captured in a CUDA Graph.
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
@@ -272,6 +273,13 @@ torch::Tensor w4a4_gemm_cutlass_dev(torch::Tensor xq, torch::Tensor wq, torch::T
 }
 
 // ---- 8-bit layers ---------------------------------------------------------------------
+// An uninitialised tensor on the device of `like`, straight from the allocator: these operators take a few microseconds, of
+// which a dispatched torch::empty would be one and a half.
+torch::Tensor new_like(at::IntArrayRef sizes, torch::ScalarType dtype, const torch::Tensor& like)
+{
+    return at::detail::empty_cuda(sizes, dtype, like.device(), c10::nullopt);
+}
+
 int dtype_code(const torch::Tensor& t, const char* op, const char* name, bool with_f32)
 {
     const auto d = t.scalar_type();
@@ -302,14 +310,14 @@ std::vector<int64_t> without_last(const torch::Tensor& t)
     return s;
 }
 
-std::vector<torch::Tensor> quant_int8(torch::Tensor x)
+std::vector<torch::Tensor> quant_int8(const torch::Tensor& x)
 {
     check_on(x, x, "quant_int8", "x");
     const int dt = dtype_code(x, "quant_int8", "x", true);
     TORCH_CHECK(x.dim() >= 1 && x.size(-1) > 0 && x.size(-1) % 16 == 0, "quant_int8: last dim must be a multiple of 16");
     const at::cuda::OptionalCUDAGuard guard(x.device());
-    auto q = torch::empty(x.sizes(), x.options().dtype(torch::kInt8));
-    auto s = torch::empty(without_last(x), x.options().dtype(torch::kFloat32));
+    auto q = new_like(x.sizes(), torch::kInt8, x);
+    auto s = new_like(without_last(x), torch::kFloat32, x);
     check_status(wush_quant_int8(x.data_ptr(), dt, rows_of(x), x.size(-1), q.data_ptr<int8_t>(), s.data_ptr<float>(), stream_of(x)),
                  "quant_int8");
     return {q, s};
@@ -339,7 +347,7 @@ const float* check_bias(const c10::optional<torch::Tensor>& bias, const torch::T
 torch::Tensor product_scratch(int64_t rows, int64_t experts, const torch::Tensor& like, size_t* nbytes)
 {
     *nbytes = wush_w8a8_gemm_workspace_bytes(rows, experts);
-    return *nbytes ? torch::empty({(int64_t)*nbytes}, like.options().dtype(torch::kUInt8)) : torch::Tensor();
+    return *nbytes ? new_like({(int64_t)*nbytes}, torch::kUInt8, like) : torch::Tensor();
 }
 void* ptr_or_null(const torch::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 
@@ -349,7 +357,7 @@ int out_code(torch::ScalarType d, const char* op)
     return d == torch::kHalf ? WUSH_F16 : WUSH_BF16;
 }
 
-torch::Tensor w8a8_gemm(torch::Tensor xq, torch::Tensor xs, torch::Tensor wq, torch::Tensor ws, c10::optional<torch::Tensor> bias,
+torch::Tensor w8a8_gemm(const torch::Tensor& xq, const torch::Tensor& xs, const torch::Tensor& wq, const torch::Tensor& ws, const c10::optional<torch::Tensor>& bias,
                         torch::ScalarType out_dtype)
 {
     const char* op = "w8a8_gemm";
@@ -360,7 +368,7 @@ torch::Tensor w8a8_gemm(torch::Tensor xq, torch::Tensor xs, torch::Tensor wq, to
     TORCH_CHECK(K > 0 && xq.size(-1) == K, op, ": K mismatch between xq and wq");
     const int code = out_code(out_dtype, op);
     const at::cuda::OptionalCUDAGuard guard(xq.device());
-    auto y = torch::empty(with_last(xq, N), xq.options().dtype(out_dtype));
+    auto y = new_like(with_last(xq, N), out_dtype, xq);
     size_t nbytes;
     auto work = product_scratch(xq.numel() / K, 1, xq, &nbytes);
     check_status(wush_w8a8_gemm(xq.data_ptr<int8_t>(), xs.data_ptr<float>(), wq.data_ptr<int8_t>(), ws.data_ptr<float>(),
@@ -370,7 +378,7 @@ torch::Tensor w8a8_gemm(torch::Tensor xq, torch::Tensor xs, torch::Tensor wq, to
     return y;
 }
 
-torch::Tensor w8a8_linear(torch::Tensor x, torch::Tensor wq, torch::Tensor ws, c10::optional<torch::Tensor> bias)
+torch::Tensor w8a8_linear(const torch::Tensor& x, const torch::Tensor& wq, const torch::Tensor& ws, const c10::optional<torch::Tensor>& bias)
 {
     const char* op = "w8a8_linear";
     check_on(x, x, op, "x");
@@ -381,9 +389,9 @@ torch::Tensor w8a8_linear(torch::Tensor x, torch::Tensor wq, torch::Tensor ws, c
     TORCH_CHECK(K > 0 && x.size(-1) == K, op, ": K mismatch between x and wq");
     const int64_t M = x.numel() / K;
     const at::cuda::OptionalCUDAGuard guard(x.device());
-    auto y = torch::empty(with_last(x, N), x.options());
+    auto y = new_like(with_last(x, N), x.scalar_type(), x);
     const size_t nbytes = wush_w8a8_linear_workspace_bytes(M, K);
-    auto work = torch::empty({(int64_t)nbytes}, x.options().dtype(torch::kUInt8));
+    auto work = new_like({(int64_t)nbytes}, torch::kUInt8, x);
     check_status(wush_w8a8_linear(x.data_ptr(), dt, wq.data_ptr<int8_t>(), ws.data_ptr<float>(), check_bias(bias, x, N, op), M, N, K,
                                   y.data_ptr(), work.data_ptr(), nbytes, stream_of(x)),
                  op);
@@ -412,7 +420,7 @@ Route check_route(const torch::Tensor& pos, const torch::Tensor& offsets, const 
     return {pos.size(0), pos.size(1), offsets.size(0) - 1};
 }
 
-std::vector<torch::Tensor> expert_sort(torch::Tensor ids, int64_t n_experts)
+std::vector<torch::Tensor> expert_sort(const torch::Tensor& ids, int64_t n_experts)
 {
     const char* op = "expert_sort";
     check_on(ids, ids, op, "ids");
@@ -420,15 +428,15 @@ std::vector<torch::Tensor> expert_sort(torch::Tensor ids, int64_t n_experts)
     TORCH_CHECK(ids.dim() == 2, op, ": ids must be (tokens, k)");
     TORCH_CHECK(n_experts >= 1 && n_experts <= WUSH_EXPERT_MAX, op, ": takes 1..", WUSH_EXPERT_MAX, " experts (got ", n_experts, ")");
     const at::cuda::OptionalCUDAGuard guard(ids.device());
-    auto pos = torch::empty(ids.sizes(), ids.options().dtype(torch::kInt32));
-    auto offsets = torch::empty({n_experts + 1}, ids.options().dtype(torch::kInt32));
+    auto pos = new_like(ids.sizes(), torch::kInt32, ids);
+    auto offsets = new_like({n_experts + 1}, torch::kInt32, ids);
     check_status(wush_expert_sort(ids.data_ptr(), bytes, ids.size(0), ids.size(1), n_experts, pos.data_ptr<int32_t>(),
                                   offsets.data_ptr<int32_t>(), stream_of(ids)),
                  op);
     return {pos, offsets};
 }
 
-torch::Tensor expert_gather(torch::Tensor x, torch::Tensor pos, torch::Tensor offsets)
+torch::Tensor expert_gather(const torch::Tensor& x, const torch::Tensor& pos, const torch::Tensor& offsets)
 {
     const char* op = "expert_gather";
     check_on(x, x, op, "x");
@@ -436,14 +444,14 @@ torch::Tensor expert_gather(torch::Tensor x, torch::Tensor pos, torch::Tensor of
     const Route r = check_route(pos, offsets, x, op);
     TORCH_CHECK(x.dim() == 2 && x.size(0) == r.tokens && x.size(1) >= 1, op, ": x must be (tokens, H) with the tokens of pos");
     const at::cuda::OptionalCUDAGuard guard(x.device());
-    auto rows = torch::empty({r.tokens * r.k, x.size(1)}, x.options());
+    auto rows = new_like({r.tokens * r.k, x.size(1)}, x.scalar_type(), x);
     check_status(wush_expert_gather(x.data_ptr(), dt, r.tokens, x.size(1), pos.data_ptr<int32_t>(), r.k, offsets.data_ptr<int32_t>(),
                                     r.experts, rows.data_ptr(), stream_of(x)),
                  op);
     return rows;
 }
 
-std::vector<torch::Tensor> expert_gather_quant_int8(torch::Tensor x, torch::Tensor pos, torch::Tensor offsets)
+std::vector<torch::Tensor> expert_gather_quant_int8(const torch::Tensor& x, const torch::Tensor& pos, const torch::Tensor& offsets)
 {
     const char* op = "expert_gather_quant_int8";
     check_on(x, x, op, "x");
@@ -452,8 +460,8 @@ std::vector<torch::Tensor> expert_gather_quant_int8(torch::Tensor x, torch::Tens
     TORCH_CHECK(x.dim() == 2 && x.size(0) == r.tokens && x.size(1) > 0 && x.size(1) % 16 == 0, op,
                 ": x must be (tokens, K) with the tokens of pos, K a multiple of 16");
     const at::cuda::OptionalCUDAGuard guard(x.device());
-    auto q = torch::empty({r.tokens * r.k, x.size(1)}, x.options().dtype(torch::kInt8));
-    auto s = torch::empty({r.tokens * r.k}, x.options().dtype(torch::kFloat32));
+    auto q = new_like({r.tokens * r.k, x.size(1)}, torch::kInt8, x);
+    auto s = new_like({r.tokens * r.k}, torch::kFloat32, x);
     check_status(wush_expert_gather_quant_int8(x.data_ptr(), dt, r.tokens, x.size(1), pos.data_ptr<int32_t>(), r.k,
                                                offsets.data_ptr<int32_t>(), r.experts, q.data_ptr<int8_t>(), s.data_ptr<float>(),
                                                stream_of(x)),
@@ -468,7 +476,7 @@ void check_weights(const torch::Tensor& w, const torch::Tensor& pos, const torch
     TORCH_CHECK(w.sizes() == pos.sizes(), op, ": weights must be (tokens, k)");
 }
 
-torch::Tensor expert_combine(torch::Tensor rows, torch::Tensor pos, c10::optional<torch::Tensor> weights)
+torch::Tensor expert_combine(const torch::Tensor& rows, const torch::Tensor& pos, const c10::optional<torch::Tensor>& weights)
 {
     const char* op = "expert_combine";
     check_on(rows, rows, op, "rows");
@@ -479,15 +487,15 @@ torch::Tensor expert_combine(torch::Tensor rows, torch::Tensor pos, c10::optiona
     TORCH_CHECK(rows.dim() == 2 && rows.size(0) == pos.numel() && rows.size(1) >= 1, op, ": rows must be (tokens * k, H)");
     if (weights.has_value()) check_weights(*weights, pos, rows, op);
     const at::cuda::OptionalCUDAGuard guard(rows.device());
-    auto y = torch::empty({pos.size(0), rows.size(1)}, rows.options());
+    auto y = new_like({pos.size(0), rows.size(1)}, rows.scalar_type(), rows);
     check_status(wush_expert_combine(rows.data_ptr(), dt, pos.size(0), rows.size(1), pos.data_ptr<int32_t>(), pos.size(1),
                                      weights.has_value() ? weights->data_ptr<float>() : nullptr, y.data_ptr(), stream_of(rows)),
                  op);
     return y;
 }
 
-std::vector<torch::Tensor> expert_combine_grad(torch::Tensor dy, torch::Tensor rows, torch::Tensor pos, torch::Tensor offsets,
-                                               torch::Tensor weights)
+std::vector<torch::Tensor> expert_combine_grad(const torch::Tensor& dy, const torch::Tensor& rows, const torch::Tensor& pos, const torch::Tensor& offsets,
+                                               const torch::Tensor& weights)
 {
     const char* op = "expert_combine_grad";
     check_on(rows, rows, op, "rows");
@@ -499,8 +507,8 @@ std::vector<torch::Tensor> expert_combine_grad(torch::Tensor dy, torch::Tensor r
     TORCH_CHECK(dy.dim() == 2 && dy.size(0) == r.tokens && dy.size(1) == rows.size(1), op, ": dy must be (tokens, H)");
     check_weights(weights, pos, rows, op);
     const at::cuda::OptionalCUDAGuard guard(rows.device());
-    auto d_rows = torch::empty_like(rows);
-    auto d_weights = torch::empty_like(weights);
+    auto d_rows = new_like(rows.sizes(), rows.scalar_type(), rows);
+    auto d_weights = new_like(weights.sizes(), weights.scalar_type(), weights);
     check_status(wush_expert_combine_grad(dy.data_ptr(), rows.data_ptr(), dt, r.tokens, rows.size(1), pos.data_ptr<int32_t>(), r.k,
                                           offsets.data_ptr<int32_t>(), r.experts, weights.data_ptr<float>(), d_rows.data_ptr(),
                                           d_weights.data_ptr<float>(), stream_of(rows)),
@@ -524,14 +532,14 @@ Grouped check_grouped(const torch::Tensor& xq, const torch::Tensor& xs, const to
     return {xq.size(0), wq.size(0), wq.size(1), xq.size(1)};
 }
 
-torch::Tensor w8a8_grouped_gemm(torch::Tensor xq, torch::Tensor xs, torch::Tensor wq, torch::Tensor ws, torch::Tensor offsets,
+torch::Tensor w8a8_grouped_gemm(const torch::Tensor& xq, const torch::Tensor& xs, const torch::Tensor& wq, const torch::Tensor& ws, const torch::Tensor& offsets,
                                 torch::ScalarType out_dtype)
 {
     const char* op = "w8a8_grouped_gemm";
     const Grouped g = check_grouped(xq, xs, wq, ws, offsets, op);
     const int code = out_code(out_dtype, op);
     const at::cuda::OptionalCUDAGuard guard(xq.device());
-    auto y = torch::empty({g.rows, g.N}, xq.options().dtype(out_dtype));
+    auto y = new_like({g.rows, g.N}, out_dtype, xq);
     size_t nbytes;
     auto work = product_scratch(g.rows, g.experts, xq, &nbytes);
     check_status(wush_w8a8_grouped_gemm(xq.data_ptr<int8_t>(), xs.data_ptr<float>(), wq.data_ptr<int8_t>(), ws.data_ptr<float>(),
@@ -541,13 +549,13 @@ torch::Tensor w8a8_grouped_gemm(torch::Tensor xq, torch::Tensor xs, torch::Tenso
     return y;
 }
 
-torch::Tensor w8a8_grouped_gated(torch::Tensor xq, torch::Tensor xs, torch::Tensor wq, torch::Tensor ws, torch::Tensor offsets)
+torch::Tensor w8a8_grouped_gated(const torch::Tensor& xq, const torch::Tensor& xs, const torch::Tensor& wq, const torch::Tensor& ws, const torch::Tensor& offsets)
 {
     const char* op = "w8a8_grouped_gated";
     const Grouped g = check_grouped(xq, xs, wq, ws, offsets, op);
     TORCH_CHECK(g.N % 2 == 0, op, ": wq must be (experts, 2 * I, K), the gate channels first");
     const at::cuda::OptionalCUDAGuard guard(xq.device());
-    auto h = torch::empty({g.rows, g.N / 2}, xq.options().dtype(torch::kFloat32));
+    auto h = new_like({g.rows, g.N / 2}, torch::kFloat32, xq);
     size_t nbytes;
     auto work = product_scratch(g.rows, g.experts, xq, &nbytes);
     check_status(wush_w8a8_grouped_gated(xq.data_ptr<int8_t>(), xs.data_ptr<float>(), wq.data_ptr<int8_t>(), ws.data_ptr<float>(),
@@ -557,8 +565,8 @@ torch::Tensor w8a8_grouped_gated(torch::Tensor xq, torch::Tensor xs, torch::Tens
     return h;
 }
 
-torch::Tensor w8a8_expert_ffn(torch::Tensor x, torch::Tensor ids, torch::Tensor weights, torch::Tensor w13q, torch::Tensor w13s,
-                              torch::Tensor w2q, torch::Tensor w2s)
+torch::Tensor w8a8_expert_ffn(const torch::Tensor& x, const torch::Tensor& ids, const torch::Tensor& weights, const torch::Tensor& w13q, const torch::Tensor& w13s,
+                              const torch::Tensor& w2q, const torch::Tensor& w2s)
 {
     const char* op = "w8a8_expert_ffn";
     check_on(x, x, op, "x");
@@ -575,9 +583,9 @@ torch::Tensor w8a8_expert_ffn(torch::Tensor x, torch::Tensor ids, torch::Tensor 
     const int64_t E = w13q.size(0), I = w13q.size(1) / 2;
     TORCH_CHECK(w2q.dim() == 3 && w2q.size(0) == E && w2q.size(1) == H && w2q.size(2) == I, op, ": w2q must be (experts, H, I)");
     const at::cuda::OptionalCUDAGuard guard(x.device());
-    auto y = torch::empty_like(x);
+    auto y = new_like(x.sizes(), x.scalar_type(), x);
     const size_t nbytes = wush_w8a8_expert_ffn_workspace_bytes(T, H, I, E, k);
-    auto work = torch::empty({(int64_t)nbytes}, x.options().dtype(torch::kUInt8));
+    auto work = new_like({(int64_t)nbytes}, torch::kUInt8, x);
     check_status(wush_w8a8_expert_ffn(x.data_ptr(), dt, ids.data_ptr(), bytes, weights.data_ptr<float>(), w13q.data_ptr<int8_t>(),
                                       w13s.data_ptr<float>(), w2q.data_ptr<int8_t>(), w2s.data_ptr<float>(), T, H, I, E, k, y.data_ptr(),
                                       work.data_ptr(), nbytes, stream_of(x)),
