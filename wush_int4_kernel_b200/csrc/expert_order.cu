@@ -183,7 +183,8 @@ int launch_sort(const Id* ids, int64_t n, int E, int32_t* pos, int32_t* offsets,
 }
 
 // ---- moves -----------------------------------------------------------------------------------------------------------------
-// V: what one thread moves at once (16 bytes where the row length and the pointers allow it, else one element).
+// A thread moves Packs of 16 bytes where the row length and the pointers allow it, of 4 bytes or one element else; of the
+// narrow ones it takes several at once, so that as many bytes are in flight.
 template <typename T> __device__ __forceinline__ float to_f32(T v);
 template <> __device__ __forceinline__ float to_f32(float v) { return v; }
 template <> __device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
@@ -194,12 +195,13 @@ template <> __device__ __forceinline__ __half from_f32(float v) { return __float
 template <> __device__ __forceinline__ __nv_bfloat16 from_f32(float v) { return __float2bfloat16_rn(v); }
 
 template <typename T, int N> struct alignas(sizeof(T) * N) Pack { T v[N]; };
+template <typename T, int N> __host__ __device__ constexpr int steps_at_once() { return sizeof(T) * N <= 4 ? 4 : 1; }
 
 // Row of an entry, or -1.  Positions come from the caller: one outside the rows counts as no row, so that nothing is
 // read or written out of range.
-__device__ __forceinline__ int64_t row_of(const int32_t* pos, int64_t i, int64_t total)
+__device__ __forceinline__ int row_of(const int32_t* pos, int64_t i, int64_t total)
 {
-    const int64_t at = pos[i];
+    const int at = pos[i];
     return at < total ? at : -1;
 }
 
@@ -222,11 +224,17 @@ __global__ void __launch_bounds__(256) expert_gather_kernel(const Pack<T, N>* __
     pdl_launch_dependents();
     const int64_t t = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
     if (t < tokens) {
-        for (int v = threadIdx.x; v < n_vec; v += blockDim.x) {
-            const Pack<T, N> p = x[t * n_vec + v];
+        constexpr int U = steps_at_once<T, N>();
+        for (int v = threadIdx.x; v < n_vec; v += U * blockDim.x) {
+            Pack<T, N> p[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) p[u] = x[t * n_vec + min(v + u * (int)blockDim.x, n_vec - 1)];
             for (int j = 0; j < k; ++j) {
                 const int64_t at = row_of(pos, t * k + j, tokens * k);
-                if (at >= 0) rows[at * n_vec + v] = p;
+                if (at < 0) continue;
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+                    if (v + u * (int)blockDim.x < n_vec) rows[at * n_vec + v + u * (int)blockDim.x] = p[u];
             }
         }
     }
@@ -234,10 +242,12 @@ __global__ void __launch_bounds__(256) expert_gather_kernel(const Pack<T, N>* __
 }
 
 // AT entries of a token at once: their rows are loaded together.  An absent entry loads row 0 and adds nothing: a branch
-// around each load would make them wait for one another (k = 8, 16384 x 4096 bf16: 563 us with branches, 222 without).
+// around each load would make them wait for one another (k = 8, 16384 x 4096 bf16: 563 us with branches, 222 without).  The
+// kernels below bound their registers so that three or four blocks share a multiprocessor (the same: 187 us with three, 212
+// with four, which spills, 221 with two; k = 4, 8192 x 4096 fp16: 56 us with four, 63 with three).
 template <typename T, int N, int AT>
 struct Entries {
-    int64_t at[AT];
+    int at[AT];
     float w[AT];
 
     __device__ __forceinline__ void load(const int32_t* pos, const float* weights, int64_t t, int k, int j0, int64_t total)
@@ -249,22 +259,33 @@ struct Entries {
             w[j] = there && weights ? weights[t * k + j0 + j] : 1.f;
         }
     }
-    __device__ __forceinline__ void add(const Pack<T, N>* rows, int64_t n_vec, int64_t v, float (&acc)[N]) const
+    // Packs v, v + stride, ... of every entry's row (the last pack where a row has fewer).
+    template <int U>
+    __device__ __forceinline__ void fetch(const Pack<T, N>* rows, int n_vec, int v, int stride, Pack<T, N> (&p)[U][AT]) const
     {
-        Pack<T, N> p[AT];
 #pragma unroll
-        for (int j = 0; j < AT; ++j) p[j] = rows[(at[j] < 0 ? 0 : at[j]) * n_vec + v];
+        for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int j = 0; j < AT; ++j)
-            if (at[j] >= 0) {
+            for (int j = 0; j < AT; ++j) p[u][j] = rows[(int64_t)max(at[j], 0) * n_vec + (U == 1 ? v : min(v + u * stride, n_vec - 1))];
+    }
+    template <int U>
+    __device__ __forceinline__ void add(const Pack<T, N>* rows, int n_vec, int v, int stride, float (&acc)[U][N]) const
+    {
+        Pack<T, N> p[U][AT];
+        fetch<U>(rows, n_vec, v, stride, p);
 #pragma unroll
-                for (int i = 0; i < N; ++i) acc[i] = __fmaf_rn(w[j], to_f32<T>(p[j].v[i]), acc[i]);
-            }
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int j = 0; j < AT; ++j)
+                if (at[j] >= 0) {
+#pragma unroll
+                    for (int i = 0; i < N; ++i) acc[u][i] = __fmaf_rn(w[j], to_f32<T>(p[u][j].v[i]), acc[u][i]);
+                }
     }
 };
 
 template <typename T, int N, int AT>
-__global__ void __launch_bounds__(256) expert_combine_kernel(const Pack<T, N>* __restrict__ rows, int64_t tokens, int n_vec,
+__global__ void __launch_bounds__(256, AT <= 4 ? 4 : 3) expert_combine_kernel(const Pack<T, N>* __restrict__ rows, int64_t tokens, int n_vec,
                                                              const int32_t* __restrict__ pos, int k,
                                                              const float* __restrict__ weights, Pack<T, N>* __restrict__ y)
 {
@@ -275,73 +296,80 @@ __global__ void __launch_bounds__(256) expert_combine_kernel(const Pack<T, N>* _
     pdl_wait();
     pdl_launch_dependents();
     if (t >= tokens) return;
-    for (int v = threadIdx.x; v < n_vec; v += blockDim.x) {
-        float acc[N];
+    constexpr int U = steps_at_once<T, N>();
+    for (int v = threadIdx.x; v < n_vec; v += U * blockDim.x) {
+        float acc[U][N];
 #pragma unroll
-        for (int i = 0; i < N; ++i) acc[i] = 0.f;
-        first.add(rows, n_vec, v, acc);
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int i = 0; i < N; ++i) acc[u][i] = 0.f;
+        first.template add<U>(rows, n_vec, v, blockDim.x, acc);
         for (int j0 = AT; j0 < k; j0 += AT) {
             Entries<T, N, AT> more;
             more.load(pos, weights, t, k, j0, tokens * k);
-            more.add(rows, n_vec, v, acc);
+            more.template add<U>(rows, n_vec, v, blockDim.x, acc);
         }
-        Pack<T, N> o;
 #pragma unroll
-        for (int i = 0; i < N; ++i) o.v[i] = from_f32<T>(acc[i]);
-        y[t * n_vec + v] = o;
+        for (int u = 0; u < U; ++u)
+            if (v + u * (int)blockDim.x < n_vec) {
+                Pack<T, N> o;
+#pragma unroll
+                for (int i = 0; i < N; ++i) o.v[i] = from_f32<T>(acc[u][i]);
+                y[t * n_vec + v + u * (int)blockDim.x] = o;
+            }
     }
 }
 
-// One block per token: dy is read once per chunk of entries, the dot products end in a block sum in a fixed order.
-template <typename T, int N>
-__global__ void __launch_bounds__(256) expert_combine_grad_kernel(const Pack<T, N>* __restrict__ dy, const Pack<T, N>* __restrict__ rows,
+// One block per token: dy is read once for every AT entries, the dot products end in a block sum in a fixed order.
+template <typename T, int N, int AT>
+__global__ void __launch_bounds__(256, AT <= 4 || steps_at_once<T, N>() > 1 ? 4 : 3) expert_combine_grad_kernel(const Pack<T, N>* __restrict__ dy, const Pack<T, N>* __restrict__ rows,
                                                                   int64_t tokens, int n_vec, const int32_t* __restrict__ pos, int k,
                                                                   const float* __restrict__ weights,
                                                                   const int32_t* __restrict__ n_used, Pack<T, N>* __restrict__ d_rows,
                                                                   float* __restrict__ d_w)
 {
-    constexpr int AT_ONCE = 4;
-    __shared__ float part[AT_ONCE][8];
+    constexpr int U = AT <= 4 ? steps_at_once<T, N>() : (steps_at_once<T, N>() + 1) / 2;
+    __shared__ float part[AT][8];
     pdl_wait();
     pdl_launch_dependents();
     const int64_t t = blockIdx.x;
-    const int tid = threadIdx.x, warps = blockDim.x >> 5;
-    for (int j0 = 0; j0 < k; j0 += AT_ONCE) {
-        int64_t at[AT_ONCE];
-        float w[AT_ONCE], dot[AT_ONCE];
+    const int tid = threadIdx.x, warps = blockDim.x >> 5, stride = blockDim.x;
+    for (int j0 = 0; j0 < k; j0 += AT) {
+        Entries<T, N, AT> en;
+        en.load(pos, weights, t, k, j0, tokens * k);
+        float dot[AT];
 #pragma unroll
-        for (int j = 0; j < AT_ONCE; ++j) {
-            at[j] = j0 + j < k ? row_of(pos, t * k + j0 + j, tokens * k) : -1;
-            w[j] = at[j] >= 0 ? weights[t * k + j0 + j] : 0.f;
-            dot[j] = 0.f;
-        }
-        for (int v = tid; v < n_vec; v += blockDim.x) {
-            const Pack<T, N> g = dy[t * n_vec + v];
-            Pack<T, N> p[AT_ONCE];
+        for (int j = 0; j < AT; ++j) dot[j] = 0.f;
+        for (int v = tid; v < n_vec; v += U * stride) {
+            Pack<T, N> g[U], p[U][AT];
 #pragma unroll
-            for (int j = 0; j < AT_ONCE; ++j)
-                if (at[j] >= 0) p[j] = rows[at[j] * n_vec + v];
+            for (int u = 0; u < U; ++u) g[u] = dy[t * n_vec + (U == 1 ? v : min(v + u * stride, n_vec - 1))];
+            en.template fetch<U>(rows, n_vec, v, stride, p);
 #pragma unroll
-            for (int j = 0; j < AT_ONCE; ++j)
-                if (at[j] >= 0) {
-                    Pack<T, N> o;
+            for (int u = 0; u < U; ++u) {
+                const bool inside = U == 1 || v + u * stride < n_vec;
 #pragma unroll
-                    for (int i = 0; i < N; ++i) {
-                        const float gi = to_f32<T>(g.v[i]);
-                        dot[j] = __fmaf_rn(gi, to_f32<T>(p[j].v[i]), dot[j]);
-                        o.v[i] = from_f32<T>(__fmul_rn(w[j], gi));
+                for (int j = 0; j < AT; ++j)
+                    if (inside && en.at[j] >= 0) {
+                        Pack<T, N> o;
+#pragma unroll
+                        for (int i = 0; i < N; ++i) {
+                            const float gi = to_f32<T>(g[u].v[i]);
+                            dot[j] = __fmaf_rn(gi, to_f32<T>(p[u][j].v[i]), dot[j]);
+                            o.v[i] = from_f32<T>(__fmul_rn(en.w[j], gi));
+                        }
+                        d_rows[(int64_t)en.at[j] * n_vec + v + u * stride] = o;
                     }
-                    d_rows[at[j] * n_vec + v] = o;
-                }
+            }
         }
 #pragma unroll
-        for (int j = 0; j < AT_ONCE; ++j) {
+        for (int j = 0; j < AT; ++j) {
 #pragma unroll
             for (int d = 16; d; d >>= 1) dot[j] += __shfl_xor_sync(0xffffffffu, dot[j], d);
             if ((tid & 31) == 0) part[j][tid >> 5] = dot[j];
         }
         __syncthreads();
-        if (tid < AT_ONCE && j0 + tid < k) {
+        if (tid < AT && j0 + tid < k) {
             float sum = 0.f;
             for (int i = 0; i < warps; ++i) sum += part[tid][i];
             d_w[t * k + j0 + tid] = sum;
@@ -351,47 +379,68 @@ __global__ void __launch_bounds__(256) expert_combine_grad_kernel(const Pack<T, 
     zero_tail(d_rows, n_vec, *n_used, tokens * k, blockIdx.x, gridDim.x, tid, blockDim.x);
 }
 
-// Threads along a row: of 32, 64, 128, 256 the count that leaves the fewest idle in the last step, the largest of equals.
-int threads_along(int64_t n_vec)
+// Threads along a row of n_vec packs of which a thread takes `at_once`: of 32, 64, 128, 256 the count that leaves the fewest
+// idle in the last step, the largest of equals.
+int threads_along(int64_t n_vec, int at_once)
 {
+    const int64_t n = (n_vec + at_once - 1) / at_once;
     int best = 32;
-    int64_t cost = (n_vec + 31) / 32 * 32;
+    int64_t cost = (n + 31) / 32 * 32;
     for (int t = 64; t <= 256; t *= 2) {
-        const int64_t c = (n_vec + t - 1) / t * t;
+        const int64_t c = (n + t - 1) / t * t;
         if (c <= cost) { best = t; cost = c; }
     }
     return best;
 }
 
-// Calls f with a Pack type: 16 bytes if the rows and the pointers allow it, else one element.
+// Calls f with the widest Pack type (16 bytes, 4 bytes, one element) that the rows and the pointers (`align`: 16, 4 or less)
+// allow.
 template <typename T, typename F>
-int with_pack(bool wide, F f)
+int with_pack(int align, F f)
 {
-    if (wide) return f(Pack<T, 16 / sizeof(T)>{});
+    if (align >= 16) return f(Pack<T, 16 / sizeof(T)>{});
+    if constexpr (sizeof(T) == 2)
+        if (align >= 4) return f(Pack<T, 2>{});
     return f(Pack<T, 1>{});
 }
 template <typename F>
-int with_type(int dtype, bool wide, F f)
+int with_type(int dtype, int align, F f)
 {
     switch (dtype) {
-        case WUSH_BF16: return with_pack<__nv_bfloat16>(wide, f);
-        case WUSH_F16: return with_pack<__half>(wide, f);
-        default: return with_pack<float>(wide, f);
+        case WUSH_BF16: return with_pack<__nv_bfloat16>(align, f);
+        case WUSH_F16: return with_pack<__half>(align, f);
+        default: return with_pack<float>(align, f);
     }
 }
-template <typename T, int N> constexpr int pack_size(const Pack<T, N>&) { return N; }
 int64_t dtype_bytes(int dtype) { return dtype == WUSH_F32 ? 4 : 2; }
-bool wide_rows(int dtype, int64_t H, const void* a, const void* b, const void* c)
+int common_align(int dtype, int64_t H, const void* a, const void* b, const void* c)
 {
-    return (H * dtype_bytes(dtype)) % 16 == 0 && aligned16(a) && aligned16(b) && aligned16(c);
+    const uintptr_t all = (uintptr_t)(H * dtype_bytes(dtype)) | (uintptr_t)a | (uintptr_t)b | (uintptr_t)c;
+    return all % 16 == 0 ? 16 : all % 4 == 0 ? 4 : 1;
 }
 bool element_aligned(int dtype, const void* p) { return (reinterpret_cast<uintptr_t>(p) & (uintptr_t)(dtype_bytes(dtype) - 1)) == 0; }
+
+// Calls f with the number of entries that a thread takes at once: all k of a token up to 8, else 8 after 8.
+template <typename F>
+int with_count(int k, F f)
+{
+    switch (k) {
+        case 1: return f(std::integral_constant<int, 1>{});
+        case 2: return f(std::integral_constant<int, 2>{});
+        case 3: return f(std::integral_constant<int, 3>{});
+        case 4: return f(std::integral_constant<int, 4>{});
+        case 5: return f(std::integral_constant<int, 5>{});
+        case 6: return f(std::integral_constant<int, 6>{});
+        case 7: return f(std::integral_constant<int, 7>{});
+    }
+    return f(std::integral_constant<int, 8>{});
+}
 
 template <typename T, int N>
 int launch_gather(Pack<T, N>, const void* x, int64_t tokens, int64_t H, const int32_t* pos, int k, const int32_t* n_used, void* rows,
                   cudaStream_t st)
 {
-    const int n_vec = (int)(H / N), tx = threads_along(n_vec), ty = 256 / tx;
+    const int n_vec = (int)(H / N), tx = threads_along(n_vec, steps_at_once<T, N>()), ty = 256 / tx;
     expert_gather_kernel<T, N><<<(unsigned)((tokens + ty - 1) / ty), dim3(tx, ty), 0, st>>>((const Pack<T, N>*)x, tokens, n_vec, pos, k,
                                                                                         n_used, (Pack<T, N>*)rows);
     return check_launch("expert_gather");
@@ -400,7 +449,7 @@ template <typename T, int N, int AT>
 int launch_combine_at(const void* rows, int64_t tokens, int64_t H, const int32_t* pos, int k, const float* weights, void* y,
                       bool dependent, cudaStream_t st)
 {
-    const int n_vec = (int)(H / N), tx = threads_along(n_vec), ty = 256 / tx;
+    const int n_vec = (int)(H / N), tx = threads_along(n_vec, steps_at_once<T, N>()), ty = 256 / tx;
     const dim3 grid((unsigned)((tokens + ty - 1) / ty)), block(tx, ty);
     if (dependent) {
         cudaError_t e = launch_dependent(expert_combine_kernel<T, N, AT>, grid, block, 0, st, (const Pack<T, N>*)rows, tokens, n_vec, pos, k,
@@ -415,25 +464,26 @@ template <typename T, int N>
 int launch_combine(Pack<T, N>, const void* rows, int64_t tokens, int64_t H, const int32_t* pos, int k, const float* weights, void* y,
                    bool dependent, cudaStream_t st)
 {
-    switch (k) {
-        case 1: return launch_combine_at<T, N, 1>(rows, tokens, H, pos, k, weights, y, dependent, st);
-        case 2: return launch_combine_at<T, N, 2>(rows, tokens, H, pos, k, weights, y, dependent, st);
-        case 3: return launch_combine_at<T, N, 3>(rows, tokens, H, pos, k, weights, y, dependent, st);
-        case 4: return launch_combine_at<T, N, 4>(rows, tokens, H, pos, k, weights, y, dependent, st);
-        case 5: return launch_combine_at<T, N, 5>(rows, tokens, H, pos, k, weights, y, dependent, st);
-        case 6: return launch_combine_at<T, N, 6>(rows, tokens, H, pos, k, weights, y, dependent, st);
-        case 7: return launch_combine_at<T, N, 7>(rows, tokens, H, pos, k, weights, y, dependent, st);
-    }
-    return launch_combine_at<T, N, 8>(rows, tokens, H, pos, k, weights, y, dependent, st);
+    return with_count(k, [&](auto at) {
+        return launch_combine_at<T, N, decltype(at)::value>(rows, tokens, H, pos, k, weights, y, dependent, st);
+    });
+}
+template <typename T, int N, int AT>
+int launch_grad_at(const void* dy, const void* rows, int64_t tokens, int64_t H, const int32_t* pos, int k, const float* weights,
+                   const int32_t* n_used, void* d_rows, float* d_w, cudaStream_t st)
+{
+    const int n_vec = (int)(H / N);
+    expert_combine_grad_kernel<T, N, AT><<<(unsigned)tokens, threads_along(n_vec, steps_at_once<T, N>()), 0, st>>>(
+        (const Pack<T, N>*)dy, (const Pack<T, N>*)rows, tokens, n_vec, pos, k, weights, n_used, (Pack<T, N>*)d_rows, d_w);
+    return check_launch("expert_combine_grad");
 }
 template <typename T, int N>
 int launch_grad(Pack<T, N>, const void* dy, const void* rows, int64_t tokens, int64_t H, const int32_t* pos, int k, const float* weights,
                 const int32_t* n_used, void* d_rows, float* d_w, cudaStream_t st)
 {
-    const int n_vec = (int)(H / N);
-    expert_combine_grad_kernel<T, N><<<(unsigned)tokens, threads_along(n_vec), 0, st>>>(
-        (const Pack<T, N>*)dy, (const Pack<T, N>*)rows, tokens, n_vec, pos, k, weights, n_used, (Pack<T, N>*)d_rows, d_w);
-    return check_launch("expert_combine_grad");
+    return with_count(k, [&](auto at) {
+        return launch_grad_at<T, N, decltype(at)::value>(dy, rows, tokens, H, pos, k, weights, n_used, d_rows, d_w, st);
+    });
 }
 
 int check_moves(const char* op, int dtype, int64_t tokens, int64_t H)
@@ -467,7 +517,7 @@ int expert_sort_launch(const void* ids, int id_bytes, int64_t n, int n_experts, 
 int expert_combine_launch(const void* rows, int dtype, int64_t tokens, int64_t H, const int32_t* pos, int k, const float* weights,
                           void* y, bool dependent, cudaStream_t st)
 {
-    return with_type(dtype, wide_rows(dtype, H, rows, y, y),
+    return with_type(dtype, common_align(dtype, H, rows, y, y),
                      [&](auto p) { return launch_combine(p, rows, tokens, H, pos, k, weights, y, dependent, st); });
 }
 
@@ -497,7 +547,7 @@ WUSH_API int wush_expert_gather(const void* x, int dtype, int64_t tokens, int64_
     WUSH_REQUIRE(element_aligned(dtype, x) && element_aligned(dtype, rows) && aligned4(pos) && aligned4(offsets),
                  "expert_gather: misaligned pointer");
     if (int e = ensure_init()) return e;
-    return with_type(dtype, wide_rows(dtype, H, x, rows, rows), [&](auto p) {
+    return with_type(dtype, common_align(dtype, H, x, rows, rows), [&](auto p) {
         return launch_gather(p, x, tokens, H, pos, (int)k, offsets + n_experts, rows, (cudaStream_t)stream);
     });
 }
@@ -529,7 +579,7 @@ WUSH_API int wush_expert_combine_grad(const void* dy, const void* rows, int dtyp
                      aligned4(offsets) && aligned4(weights) && aligned4(d_weights),
                  "expert_combine_grad: misaligned pointer");
     if (int e = ensure_init()) return e;
-    return with_type(dtype, wide_rows(dtype, H, dy, rows, d_rows), [&](auto p) {
+    return with_type(dtype, common_align(dtype, H, dy, rows, d_rows), [&](auto p) {
         return launch_grad(p, dy, rows, tokens, H, pos, (int)k, weights, offsets + n_experts, d_rows, d_weights, (cudaStream_t)stream);
     });
 }
