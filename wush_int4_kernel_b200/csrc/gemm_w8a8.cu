@@ -560,9 +560,10 @@ __global__ void __launch_bounds__(THREADS, 1) w8a8_stream_kernel(const __grid_co
 // of a stage, two accumulators rotate in tensor memory so the epilogue of a tile runs under the MMAs of the next, and the
 // pairs are persistent.  The token count of a tile is a multiple of 32 chosen per expert (its rows in equal tiles), so a
 // ragged expert costs MMAs for at most 31 rows that do not exist, not for a full tile.
-constexpr int PAIR_TOKENS = 256, PAIR_STAGES = 6, PAIR_ACC = 2;
+constexpr int PAIR_TOKENS = 256, PAIR_STAGES = 3, PAIR_BLOCKS = 2, PAIR_ACC = 2;
 constexpr int PAIR_EPILOGUE = 256, PAIR_THREADS = 64 + PAIR_EPILOGUE;     // eight epilogue warps: two share a quarter of the lanes
-constexpr int PAIR_STAGE = 2 * A_BYTES;                  // 128 weight rows and up to 128 token rows
+constexpr int PAIR_BLOCK = 2 * A_BYTES;                  // 128 bytes of 128 weight rows and of up to 128 token rows
+constexpr int PAIR_STAGE = PAIR_BLOCKS * PAIR_BLOCK;
 constexpr int PAIR_SX = PAIR_STAGES * PAIR_STAGE;        // token scales of two tiles
 constexpr int PAIR_TABLE = PAIR_SX + 2 * PAIR_TOKENS * 4;
 constexpr int PAIR_TABLE_BYTES = 2 * (WUSH_EXPERT_MAX + 2) * 4;
@@ -667,7 +668,7 @@ w8a8_pair_kernel(const __grid_constant__ PairMaps maps, const Params p, int band
     const uint32_t tmem = *tmem_slot;
     const int n_tiles = p.offsets ? first_s[p.experts] : token_tiles((int)p.rows) * p.tiles_c;
     TileOrder order = {p, p.offsets ? first_s : nullptr, row_s, band, p.offsets ? expert_of_tile(p, first_s, pair) : 0};
-    const int k_steps = (p.K + 127) / 128;
+    const int k_blocks = (p.K + 127) / 128, k_steps = (k_blocks + PAIR_BLOCKS - 1) / PAIR_BLOCKS;
     constexpr int WIDTH = GATED ? 64 : 128;              // channels of the result per CTA
 
     if (warp == 0) {
@@ -685,9 +686,12 @@ w8a8_pair_kernel(const __grid_constant__ PairMaps maps, const Params p, int band
                     if (!tc::mbar_wait(&empty[slot], phase ^ 1)) { ok = false; break; }
                     uint8_t* st = smem + slot * PAIR_STAGE;
                     const uint32_t bar = tc::map_to_rank(&full[slot], 0);
-                    if (rank == 0) tc::mbar_expect_tx(&full[slot], bytes);
-                    tma_load_4d_pair(st, &maps.w, bar, ks * 128, 0, c0, tile.expert);
-                    tc::tma_load_2d_pair(st + A_BYTES, mx, bar, ks * 128, row);
+                    const int blocks = min(PAIR_BLOCKS, k_blocks - ks * PAIR_BLOCKS);
+                    if (rank == 0) tc::mbar_expect_tx(&full[slot], blocks * bytes);
+                    for (int b = 0; b < blocks; ++b) {
+                        tma_load_4d_pair(st + b * PAIR_BLOCK, &maps.w, bar, (ks * PAIR_BLOCKS + b) * 128, 0, c0, tile.expert);
+                        tc::tma_load_2d_pair(st + b * PAIR_BLOCK + A_BYTES, mx, bar, (ks * PAIR_BLOCKS + b) * 128, row);
+                    }
                     ++issued;
                     if (++slot == PAIR_STAGES) { slot = 0; phase ^= 1; }
                 }
@@ -716,14 +720,17 @@ w8a8_pair_kernel(const __grid_constant__ PairMaps maps, const Params p, int band
                 for (int ks = 0; ks < k_steps; ++ks) {
                     if (!tc::mbar_wait(&full[slot], phase)) { ok = false; break; }
                     tc::tc_fence_after();
-                    const uint32_t sa = tc::smem_u32(smem + slot * PAIR_STAGE), sb = sa + A_BYTES;
+                    const int blocks = min(PAIR_BLOCKS, k_blocks - ks * PAIR_BLOCKS);
+                    for (int b = 0; b < blocks; ++b) {
+                        const uint32_t sa = tc::smem_u32(smem + slot * PAIR_STAGE + b * PAIR_BLOCK), sb = sa + A_BYTES;
 #pragma unroll
-                    for (int kk = 0; kk < 4; ++kk)
-                        tc::mma_i8_pair(tmem + ab * PAIR_TOKENS, desc_sw128(sa + kk * 32), desc_sw128(sb + kk * 32), idesc, (ks | kk) ? 1u : 0u);
+                        for (int kk = 0; kk < 4; ++kk)
+                            tc::mma_i8_pair(tmem + ab * PAIR_TOKENS, desc_sw128(sa + kk * 32), desc_sw128(sb + kk * 32), idesc, (ks | b | kk) ? 1u : 0u);
+                    }
                     tc::mma_commit_pair(&empty[slot]);                           // frees the stage in both CTAs
                     if (++slot == PAIR_STAGES) { slot = 0; phase ^= 1; }
                     // The next tile's width, while the tensor core has stages to work on: between two tiles it would wait for it.
-                    if (ks == (k_steps > 2 ? 2 : 0) && t + n_pairs < n_tiles) next = tc::idesc_i8_pair(order.at(t + n_pairs).nt);
+                    if (ks == (k_steps > 1 ? 1 : 0) && t + n_pairs < n_tiles) next = tc::idesc_i8_pair(order.at(t + n_pairs).nt);
                 }
                 idesc = next;
                 if (!ok) break;

@@ -4,7 +4,7 @@
 // row t go to up to k other rows (an expert's batch): the row is read and quantised once and stored k times.
 //
 // Bound by memory: size(x) bytes read and one byte per element (times k) written.  A row stays in registers between
-// its maximum and its codes (32 elements per thread, at most 1024 threads: rows of up to 32768 elements; what is
+// its maximum and its codes (64 elements of 16 bits or 32 of 32 per thread, at most 1024 threads: rows of up to 65536 or 32768 elements; what is
 // beyond is read again, from L2).
 //
 // The codes of bf16 and fp16 rows are those of the definition exactly, without a division per element.  With
@@ -23,7 +23,7 @@ namespace wush {
 namespace {
 
 constexpr int VEC = 16;                  // elements per thread and step: 16 bytes of codes
-constexpr int HOLD = 2;                  // steps kept in registers
+template <typename T> constexpr int HOLD = sizeof(T) == 2 ? 4 : 2;       // steps kept in registers: 32 of them
 
 template <typename T> struct Raw16;      // 16 elements as loaded
 template <> struct Raw16<float> { uint4 w[4]; };
@@ -118,7 +118,7 @@ template <typename T>
 struct Row {
     const T* x;
     int vecs, lane, tpr;
-    Raw16<T> held[HOLD];
+    Raw16<T> held[HOLD<T>];
     float scale, inv;
     bool tiny;
 
@@ -128,12 +128,12 @@ struct Row {
         uint32_t m = 0;
         if (live) {
 #pragma unroll
-            for (int i = 0; i < HOLD; ++i)
+            for (int i = 0; i < HOLD<T>; ++i)
                 if (lane + i * tpr < vecs) held[i] = load16<T>(x + (int64_t)(lane + i * tpr) * VEC);
 #pragma unroll
-            for (int i = 0; i < HOLD; ++i)
+            for (int i = 0; i < HOLD<T>; ++i)
                 if (lane + i * tpr < vecs) m = amax_bits<T>(held[i], m);
-            for (int v = lane + HOLD * tpr; v < vecs; v += tpr) m = amax_bits<T>(load16<T>(x + (int64_t)v * VEC), m);
+            for (int v = lane + HOLD<T> * tpr; v < vecs; v += tpr) m = amax_bits<T>(load16<T>(x + (int64_t)v * VEC), m);
         }
         if constexpr (sizeof(T) == 2) m = max(m & 0xffffu, m >> 16);
         m = __reduce_max_sync(0xffffffffu, m);
@@ -156,9 +156,9 @@ struct Row {
     {
         const uint4 zero = make_uint4(0, 0, 0, 0);
 #pragma unroll
-        for (int i = 0; i < HOLD; ++i)
+        for (int i = 0; i < HOLD<T>; ++i)
             if (lane + i * tpr < vecs) put(lane + i * tpr, inv > 0.f ? codes16<T>(held[i], inv, tiny) : zero);
-        for (int v = lane + HOLD * tpr; v < vecs; v += tpr)
+        for (int v = lane + HOLD<T> * tpr; v < vecs; v += tpr)
             put(v, inv > 0.f ? codes16<T>(load16<T>(x + (int64_t)v * VEC), inv, tiny) : zero);
     }
     // Codes and scale to row r, or to the rows of k entries (those outside [0, total) are no rows).
@@ -225,10 +225,12 @@ __global__ void __launch_bounds__(1024) quant_int8_kernel(const T* __restrict__ 
     if (n_used) zero_tail(q, s, K / VEC, *n_used, rows * k);
 }
 
-// Threads per row.  Few rows: a thread for every 16 elements.  Many: two steps per thread, which the registers hold.
+// Threads per row.  Few rows: a thread for every 16 elements.  Many: as many steps per thread as the registers hold
+// (333 x 28672 bf16: QUANT_US).
+template <typename T>
 int threads_per_row(int64_t rows, int64_t K)
 {
-    const int vecs = (int)(K / VEC), want = rows <= 2 * sm_count() ? vecs : (vecs + HOLD - 1) / HOLD;
+    const int vecs = (int)(K / VEC), want = rows <= 2 * sm_count() ? vecs : (vecs + HOLD<T> - 1) / HOLD<T>;
     int tpr = 32;
     while (tpr < want && tpr < 1024) tpr *= 2;
     return tpr;
@@ -237,7 +239,7 @@ int threads_per_row(int64_t rows, int64_t K)
 template <typename T>
 int launch_quant(const QuantRows& a, bool dependent, cudaStream_t st)
 {
-    const int tpr = threads_per_row(a.rows, a.K);
+    const int tpr = threads_per_row<T>(a.rows, a.K);
     const int block = tpr < 256 ? 256 : tpr;
     const int64_t per = block / tpr, grid = (a.rows + per - 1) / per;
     if (grid > 0x7fffffffll) return fail(WUSH_ERR_UNSUPPORTED, "quant_int8: too many rows (%lld)", (long long)a.rows);
