@@ -713,6 +713,7 @@ w8a8_pair_kernel(const __grid_constant__ PairMaps maps, const Params p, int band
         if (lane == 0 && rank == 0) {
             uint32_t slot = 0, phase = 0, ab = 0, aphase = 0;
             bool ok = true;
+            const uint64_t desc0 = desc_sw128(tc::smem_u32(smem));
             uint32_t idesc = pair < n_tiles ? tc::idesc_i8_pair(order.at(pair).nt) : 0, next = 0;
             for (int t = pair; t < n_tiles && ok; t += n_pairs) {
                 if (!tc::mbar_wait(&acc_empty[ab], aphase ^ 1)) { ok = false; break; }
@@ -721,12 +722,16 @@ w8a8_pair_kernel(const __grid_constant__ PairMaps maps, const Params p, int band
                     if (!tc::mbar_wait(&full[slot], phase)) { ok = false; break; }
                     tc::tc_fence_after();
                     const int blocks = min(PAIR_BLOCKS, k_blocks - ks * PAIR_BLOCKS);
-                    for (int b = 0; b < blocks; ++b) {
-                        const uint32_t sa = tc::smem_u32(smem + slot * PAIR_STAGE + b * PAIR_BLOCK), sb = sa + A_BYTES;
+                    const uint64_t da = desc0 + (uint64_t)(slot * (PAIR_STAGE / 16));
 #pragma unroll
-                        for (int kk = 0; kk < 4; ++kk)
-                            tc::mma_i8_pair(tmem + ab * PAIR_TOKENS, desc_sw128(sa + kk * 32), desc_sw128(sb + kk * 32), idesc, (ks | b | kk) ? 1u : 0u);
-                    }
+                    for (int b = 0; b < PAIR_BLOCKS; ++b)
+                        if (b < blocks) {
+#pragma unroll
+                            for (int kk = 0; kk < 4; ++kk) {
+                                const uint64_t d = da + (b * PAIR_BLOCK + kk * 32) / 16;
+                                tc::mma_i8_pair(tmem + ab * PAIR_TOKENS, d, d + A_BYTES / 16, idesc, (ks | b | kk) ? 1u : 0u);
+                            }
+                        }
                     tc::mma_commit_pair(&empty[slot]);                           // frees the stage in both CTAs
                     if (++slot == PAIR_STAGES) { slot = 0; phase ^= 1; }
                     // The next tile's width, while the tensor core has stages to work on: between two tiles it would wait for it.
