@@ -379,6 +379,10 @@ int wush_comm_destroy(void* comm);
  * the smallest count that holds them up to 32 rows; beyond, the count minimising (blocks of rows) x
  * (measured time of a block), since every block streams the weights again.  Host only, no GPU. */
 int wush_debug_stream_tiles(int64_t M);
+/* The same for the 8-bit products: kernel 0 the streaming kernel (`ctas` CTAs), 1 the pair kernel (`ctas` pairs); cover
+ * [tiles * k_steps] ints out, added to: how many pieces cover each stage of each tile; *cut: tiles that are cut.  Returns WUSH_OK
+ * if every piece is in range and has a slot of its own and a cut tile is finished from exactly its pieces; 101..106 otherwise. */
+int wush_debug_w8a8_cover(int kernel, int tiles, int k_steps, int ctas, int* cover, int* cut);
 int wush_debug_unit_cover(int64_t tiles, int k_steps, int gran, int workers, int force_mode,
                           double step_us, double piece_us, int* cover, int slots, int* plan_out);
 

@@ -156,7 +156,9 @@ def product64(xq, xs, wq, ws):
     (1, 1, 16), (1, 128, 128), (1, 4096, 4096), (2, 130, 272), (3, 5003, 4112), (5, 640, 8192), (15, 257, 1040), (16, 1024, 512),
     (17, 1024, 512), (31, 999, 2064), (32, 256, 16384), (33, 384, 640), (63, 127, 144), (64, 8192, 1024), (65, 256, 256),
     (100, 1000, 2000), (128, 512, 512), (129, 513, 528), (255, 640, 1024), (256, 256, 256), (257, 258, 272), (300, 2048, 4096),
-    (513, 1026, 1008), (1000, 3001, 720), (2100, 512, 2048)])
+    (513, 1026, 1008), (1000, 3001, 720), (2100, 512, 2048),
+    # long K: tiles of the last wave cut along K, few of them, many of them, with narrow and odd edges
+    (65, 130, 16384), (100, 1000, 12304), (129, 513, 8192), (300, 4099, 8192), (333, 2048, 28672), (300, 20000, 6160)])
 def test_w8a8_gemm(C, M, N, K, out):
     g = gen(M * 31 + N * 7 + K)
     xq, wq = codes(M, K, g=g), codes(N, K, g=g)
@@ -447,6 +449,24 @@ def test_grouped_gated(C, sizes, tail, inner, K):
     a = 0
     for i, n in enumerate(sizes):
         g, u = product64(xq[a:a + n], xs[a:a + n], wq[i], ws[i]).chunk(2, dim=-1)
+        want = g * torch.sigmoid(g) * u
+        within(h[a:a + n], want, want.abs() * (3 * (1 + g.abs()) + 3 + 10 + 2) * U + 1e-30 * (1 + u.abs()))
+        a += n
+
+
+@pytest.mark.parametrize("sizes,tail", [([100, 0, 300, 71], 5), ([512], 0), ([1, 700], 3), ([90] * 6, 0)])
+def test_grouped_long_k(C, sizes, tail):
+    """Enough stages for the last wave's tiles to be cut along K."""
+    N, K = 520, 8208
+    xq, xs, wq, ws, offsets = grouped_case(sizes, tail, N, K, gen(sum(sizes)))
+    y = C.w8a8_grouped_gemm(xq, xs, wq, ws, offsets)
+    h = C.w8a8_grouped_gated(xq, xs, wq, ws, offsets)
+    assert not y[sum(sizes):].any() and not h[sum(sizes):].any()
+    a = 0
+    for i, n in enumerate(sizes):
+        want = product64(xq[a:a + n], xs[a:a + n], wq[i], ws[i])
+        within(y[a:a + n], want, want.abs() * (e(torch.float16) + 4 * U) + TINY16)
+        g, u = want.chunk(2, dim=-1)
         want = g * torch.sigmoid(g) * u
         within(h[a:a + n], want, want.abs() * (3 * (1 + g.abs()) + 3 + 10 + 2) * U + 1e-30 * (1 + u.abs()))
         a += n

@@ -129,3 +129,21 @@ def test_header_constants_of_the_8_bit_operators():
     assert [value("WUSH_BF16"), value("WUSH_F16"), value("WUSH_F32")] == [capi.BF16, capi.F16, capi.F32]
     assert [value("#define WUSH_W8A8_MAX_K".split()[1]), value("WUSH_EXPERT_MAX"), value("WUSH_EXPERT_MAX_K")] == \
         [capi.W8A8_MAX_K, capi.EXPERT_MAX, capi.EXPERT_MAX_K]
+
+
+def test_division_of_work_covers_every_stage_once(lib):
+    """Both kernels' pieces, walked on the host: every stage of every tile once, every piece a slot of its own."""
+    import ctypes
+    import random
+
+    rng = random.Random(5)
+    shapes = [(0, 1), (1, 1), (1, 1000), (147, 3), (148, 1), (149, 64), (448, 64), (192, 33), (64, 64), (3, 2), (1000, 9), (224, 32), (75, 31)]
+    shapes += [(int(2 ** rng.uniform(0, 12)), int(2 ** rng.uniform(0, 9))) for _ in range(400)]
+    cuts = [0, 0]
+    for kernel, ctas in ((0, 148), (1, 74), (0, 132), (1, 66)):
+        for tiles, steps in shapes:
+            cover, cut = (ctypes.c_int * max(1, tiles * steps))(), ctypes.c_int(-1)
+            assert lib.wush_debug_w8a8_cover(kernel, tiles, steps, ctas, cover, ctypes.byref(cut)) == 0, (kernel, tiles, steps, ctas)
+            assert all(v == 1 for v in cover[:tiles * steps]), (kernel, tiles, steps, ctas)
+            cuts[kernel] += cut.value
+    assert cuts[0] > 1000 and cuts[1] > 100

@@ -20,6 +20,8 @@
 // Roles per CTA (192 threads): warp 0 TMA producer, warp 1 MMA issuer (and owner of the tensor memory), warps 2-5 epilogue.
 // Every wait is bounded; one that gives up leaves a role code in a device word (wush_device_flag, bits 16-23).
 #include <algorithm>
+#include <new>
+#include <vector>
 
 #include "common.cuh"
 #include "int8_host.cuh"
@@ -60,6 +62,7 @@ struct Params {
     int early;                   // weights (and offsets) may be read before the kernel in front has finished
     int32_t* counters;           // one per CTA, zero
     uint32_t* pieces;            // two per CTA
+    int weights_once;            // pair kernel: what reads a weight does so at about the same time
 };
 
 __device__ __forceinline__ uint64_t desc_sw128(uint32_t saddr)
@@ -279,7 +282,7 @@ struct Run {
     int k_steps;
     int pieces;                  // tiles and parts of tiles in the run
 };
-__device__ __forceinline__ Run make_run(int tiles, int k_steps, int cta, int ctas)
+__host__ __device__ inline Run make_run(int tiles, int k_steps, int cta, int ctas)
 {
     Run r;
     const int total = tiles * k_steps, per = tiles / ctas, more = tiles - per * ctas;
@@ -301,7 +304,7 @@ __device__ __forceinline__ Run make_run(int tiles, int k_steps, int cta, int cta
 struct Piece {
     int t, k0, k1;
 };
-__device__ __forceinline__ Piece piece_of(const Run& r, int i)
+__host__ __device__ inline Piece piece_of(const Run& r, int i)
 {
     Piece q;
     q.t = r.begin / r.k_steps + i;
@@ -311,7 +314,7 @@ __device__ __forceinline__ Piece piece_of(const Run& r, int i)
     return q;
 }
 // The CTA of a split whose run holds `stage`.
-__device__ __forceinline__ int owner(const Run& r, int stage)
+__host__ __device__ inline int owner(const Run& r, int stage)
 {
     const int border = r.longer * (r.size + 1);
     return stage < border ? stage / (r.size + 1) : r.longer + (stage - border) / r.size;
@@ -576,6 +579,15 @@ struct PairMaps {
     CUtensorMap x[3];            // boxes of 32, 64, 128 token rows
 };
 
+__device__ __forceinline__ void tma_load_4d_pair(void* dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int c2, int c3,
+                                                 uint64_t policy)
+{
+    asm volatile(
+        "cp.async.bulk.tensor.4d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%3, %4, %5, %6}], [%2], %7;" ::"r"(
+            tc::smem_u32(dst)),
+        "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "l"(policy)
+        : "memory");
+}
 __device__ __forceinline__ void tma_load_4d_pair(void* dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int c2, int c3)
 {
     asm volatile(
@@ -588,6 +600,45 @@ __device__ __forceinline__ void tma_load_4d_pair(void* dst, const CUtensorMap* m
 // Token tiles of `count` rows: as few as possible, of equal size.  (tiles - 1) * nt < count, because nt <= 256.
 __host__ __device__ __forceinline__ int token_tiles(int count) { return (int)(((unsigned)count + PAIR_TOKENS - 1) / PAIR_TOKENS); }
 __device__ __forceinline__ int tile_width(int count, int tiles) { return tiles == 1 ? (count + 31) & ~31 : (int)((((unsigned)count + tiles - 1) / (unsigned)tiles + 31) & ~31u); }
+
+// The tiles of the last, partly filled wave are cut along K: `split` pairs take a share of the stages of one tile each and
+// leave their sums in the workspace, and a second kernel adds them and finishes the tile, on all multiprocessors (a single
+// CTA would need ten microseconds to read eight pieces).  Done where it saves more than storing, launching and adding cost:
+// TAIL_STAGES stages of about 0.6 us.  8192 x 57344: 128 rows (3.03 waves) 101 -> 93 us, 333 rows (6.05)
+// 156 -> 150; 4096 x 24576: 1024 rows (5.19) 79.4 -> 78.2, and 82.5 with TAIL_STAGES = 10.
+constexpr int TAIL_STAGES = 14, TAIL_SPLIT = 8, TAIL_TOKENS = 8;
+struct Tail {
+    int full;                    // tiles that one pair takes whole
+    int split;                   // pairs per tile behind them; 0: none is cut
+};
+__host__ __device__ inline Tail tail_plan(int n_tiles, int k_steps, int pairs, bool allowed)
+{
+    const int rest = n_tiles % pairs, split = rest ? pairs / rest : 0;
+    const int most = k_steps < TAIL_SPLIT ? k_steps : TAIL_SPLIT, share = split < most ? split : most;
+    if (allowed && share >= 2 && k_steps - (k_steps + share - 1) / share > TAIL_STAGES) return {n_tiles - rest, share};
+    return {n_tiles, 0};
+}
+// i-th piece of work of a pair: stages [k0, k1) of tile t.
+struct Work {
+    int t, k0, k1;
+    bool valid, whole;
+};
+__host__ __device__ inline Work work_of(const Tail& tail, int n_tiles, int k_steps, int pair, int pairs, int i)
+{
+    Work w;
+    w.t = pair + i * pairs;
+    w.k0 = 0;
+    w.k1 = k_steps;
+    w.valid = w.whole = w.t < tail.full;
+    if (!w.valid && tail.split && w.t < tail.full + pairs) {              // the wave behind the whole tiles
+        const int tile = pair / tail.split, part = pair - tile * tail.split;
+        w.t = tail.full + tile;
+        w.valid = w.t < n_tiles;
+        w.k0 = part * k_steps / tail.split;
+        w.k1 = (part + 1) * k_steps / tail.split;
+    }
+    return w;
+}
 
 // Tile t in the order in which the pairs take them.  Inside a group of token tiles the tokens run fastest, so tiles that
 // run together share weight rows and one wave's weights are read from HBM once.  Groups: the experts, or, with one
@@ -667,29 +718,36 @@ w8a8_pair_kernel(const __grid_constant__ PairMaps maps, const Params p, int band
     tc::tc_fence_after();
     const uint32_t tmem = *tmem_slot;
     const int n_tiles = p.offsets ? first_s[p.experts] : token_tiles((int)p.rows) * p.tiles_c;
-    TileOrder order = {p, p.offsets ? first_s : nullptr, row_s, band, p.offsets ? expert_of_tile(p, first_s, pair) : 0};
     const int k_blocks = (p.K + 127) / 128, k_steps = (k_blocks + PAIR_BLOCKS - 1) / PAIR_BLOCKS;
     constexpr int WIDTH = GATED ? 64 : 128;              // channels of the result per CTA
+    const Tail tail = tail_plan(n_tiles, k_steps, n_pairs, p.pieces != nullptr);
+    auto work = [&](int i) { return work_of(tail, n_tiles, k_steps, pair, n_pairs, i); };
+    TileOrder order = {p, p.offsets ? first_s : nullptr, row_s, band, p.offsets ? expert_of_tile(p, first_s, work(0).t) : 0};
 
     if (warp == 0) {
         if (lane == 0) {
             uint32_t slot = 0, phase = 0;
             int issued = 0;
             bool ok = true;
-            for (int t = pair; t < n_tiles && ok; t += n_pairs) {
-                const Tile tile = order.at(t);
+            const uint64_t policy = evict_first_policy();
+            for (int i = 0; ok; ++i) {
+                const Work w = work(i);
+                if (!w.valid) break;
+                const Tile tile = order.at(w.t);
                 const int half = tile.nt / 2, c0 = tile.ct * 2 * WIDTH + (int)rank * WIDTH;
                 const int m = half <= 32 ? 0 : half <= 64 ? 1 : 2, row = (int)tile.row0 + (int)rank * half;
                 const uint32_t bytes = 2 * (A_BYTES + (32 << m) * 128);          // of both CTAs
                 const CUtensorMap* mx = &maps.x[m];
-                for (int ks = 0; ks < k_steps; ++ks) {
+                for (int ks = w.k0; ks < w.k1; ++ks) {
                     if (!tc::mbar_wait(&empty[slot], phase ^ 1)) { ok = false; break; }
                     uint8_t* st = smem + slot * PAIR_STAGE;
                     const uint32_t bar = tc::map_to_rank(&full[slot], 0);
                     const int blocks = min(PAIR_BLOCKS, k_blocks - ks * PAIR_BLOCKS);
                     if (rank == 0) tc::mbar_expect_tx(&full[slot], blocks * bytes);
                     for (int b = 0; b < blocks; ++b) {
-                        tma_load_4d_pair(st + b * PAIR_BLOCK, &maps.w, bar, (ks * PAIR_BLOCKS + b) * 128, 0, c0, tile.expert);
+                        const int k = (ks * PAIR_BLOCKS + b) * 128;
+                        if (p.weights_once) tma_load_4d_pair(st + b * PAIR_BLOCK, &maps.w, bar, k, 0, c0, tile.expert, policy);
+                        else tma_load_4d_pair(st + b * PAIR_BLOCK, &maps.w, bar, k, 0, c0, tile.expert);
                         tc::tma_load_2d_pair(st + b * PAIR_BLOCK + A_BYTES, mx, bar, (ks * PAIR_BLOCKS + b) * 128, row);
                     }
                     ++issued;
@@ -714,11 +772,12 @@ w8a8_pair_kernel(const __grid_constant__ PairMaps maps, const Params p, int band
             uint32_t slot = 0, phase = 0, ab = 0, aphase = 0;
             bool ok = true;
             const uint64_t desc0 = desc_sw128(tc::smem_u32(smem));
-            uint32_t idesc = pair < n_tiles ? tc::idesc_i8_pair(order.at(pair).nt) : 0, next = 0;
-            for (int t = pair; t < n_tiles && ok; t += n_pairs) {
+            Work w = work(0), w_next = {};
+            uint32_t idesc = w.valid ? tc::idesc_i8_pair(order.at(w.t).nt) : 0, next = 0;
+            for (int i = 0; w.valid && ok; ++i) {
                 if (!tc::mbar_wait(&acc_empty[ab], aphase ^ 1)) { ok = false; break; }
                 tc::tc_fence_after();
-                for (int ks = 0; ks < k_steps; ++ks) {
+                for (int ks = w.k0; ks < w.k1; ++ks) {
                     if (!tc::mbar_wait(&full[slot], phase)) { ok = false; break; }
                     tc::tc_fence_after();
                     const int blocks = min(PAIR_BLOCKS, k_blocks - ks * PAIR_BLOCKS);
@@ -729,15 +788,19 @@ w8a8_pair_kernel(const __grid_constant__ PairMaps maps, const Params p, int band
 #pragma unroll
                             for (int kk = 0; kk < 4; ++kk) {
                                 const uint64_t d = da + (b * PAIR_BLOCK + kk * 32) / 16;
-                                tc::mma_i8_pair(tmem + ab * PAIR_TOKENS, d, d + A_BYTES / 16, idesc, (ks | b | kk) ? 1u : 0u);
+                                tc::mma_i8_pair(tmem + ab * PAIR_TOKENS, d, d + A_BYTES / 16, idesc, ((ks - w.k0) | b | kk) ? 1u : 0u);
                             }
                         }
                     tc::mma_commit_pair(&empty[slot]);                           // frees the stage in both CTAs
                     if (++slot == PAIR_STAGES) { slot = 0; phase ^= 1; }
                     // The next tile's width, while the tensor core has stages to work on: between two tiles it would wait for it.
-                    if (ks == (k_steps > 1 ? 1 : 0) && t + n_pairs < n_tiles) next = tc::idesc_i8_pair(order.at(t + n_pairs).nt);
+                    if (ks == w.k0 + (w.k1 - w.k0 > 1 ? 1 : 0)) {
+                        w_next = work(i + 1);
+                        if (w_next.valid) next = tc::idesc_i8_pair(order.at(w_next.t).nt);
+                    }
                 }
                 idesc = next;
+                w = w_next;
                 if (!ok) break;
                 tc::mma_commit_pair(&acc_full[ab]);                              // both CTAs' epilogues may read
                 if (++ab == PAIR_ACC) { ab = 0; aphase ^= 1; }
@@ -757,20 +820,23 @@ w8a8_pair_kernel(const __grid_constant__ PairMaps maps, const Params p, int band
         Tile tile = {};
         Lane L = {};
         float sx_mine = 0.f;                                                     // scale of token `me` of the tile
-        auto fetch = [&](int t) {
-            tile = order.at(t);
+        Work w = work(0);
+        auto fetch = [&]() {
+            tile = order.at(w.t);
             L = make_lane<GATED>(p, tile, (int64_t)tile.ct * 2 * WIDTH + rank * WIDTH, c, nullptr);
             sx_mine = me < tile.n_rows ? p.xs[tile.row0 + me] : 0.f;
         };
-        if (pair < n_tiles) fetch(pair);
-        for (int t = pair; t < n_tiles; t += n_pairs) {
+        if (w.valid) fetch();
+        for (int i = 0; w.valid; ++i) {
             float* sx = sx_s + ab * PAIR_TOKENS;
             if (me < tile.nt) sx[me] = sx_mine;
             asm volatile("bar.sync 1, 256;" ::: "memory");                       // the epilogue's own barrier
             Lane now = L;
             now.sx = sx;
             const int chunks = tile.nt / 32;
-            if (t + n_pairs < n_tiles) fetch(t + n_pairs);                       // the next tile's scales arrive under this one's work
+            const bool whole = w.whole;
+            w = work(i + 1);
+            if (w.valid) fetch();                                                // the next tile's scales arrive under this one's work
             if (ok) ok = __all_sync(0xffffffffu, tc::mbar_wait(&acc_full[ab], aphase));
             tc::tc_fence_after();
 #pragma unroll 1
@@ -783,7 +849,13 @@ w8a8_pair_kernel(const __grid_constant__ PairMaps maps, const Params p, int band
                     __syncwarp();
                     if (lane == 0) tc::mbar_arrive_cluster(tc::map_to_rank(&acc_empty[ab], 0));
                 }
-                emit<GATED, 32>(p, now, c0 * 32, v);
+                if (whole) {
+                    emit<GATED, 32>(p, now, c0 * 32, v);
+                } else {
+                    uint32_t* slot = p.pieces + ((size_t)blockIdx.x * PAIR_TOKENS + c0 * 32) * 128 + c;
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) __stcg(slot + j * 128, v[j]);
+                }
             }
             if (half >= chunks && lane == 0) tc::mbar_arrive_cluster(tc::map_to_rank(&acc_empty[ab], 0));
             if (++ab == PAIR_ACC) { ab = 0; aphase ^= 1; }
@@ -797,6 +869,52 @@ w8a8_pair_kernel(const __grid_constant__ PairMaps maps, const Params p, int band
     __syncthreads();
     tc::cluster_sync_all();
     if (warp == 1) tc::tmem_dealloc_pair(tmem, 512);
+}
+
+// Adds the pieces of the tiles that the pair kernel cut and finishes them: a block for 8 tokens of the 128 weight rows of one
+// CTA, four pieces loaded at once (32 tokens, one piece after another: M = 128 above took 124 us).  `pairs`: of the launch in
+// front.
+template <bool GATED>
+__global__ void __launch_bounds__(128) w8a8_tail_kernel(const Params p, int band, int pairs)
+{
+    __shared__ int32_t first_s[WUSH_EXPERT_MAX + 2], row_s[WUSH_EXPERT_MAX + 2];
+    __shared__ alignas(16) float sx_s[TAIL_TOKENS];
+    pdl_wait();
+    pdl_launch_dependents();
+    const int c = threadIdx.x;
+    if (p.offsets) {
+        if (c < 32) make_table(p, first_s, row_s, [](int n) { return token_tiles(n); });
+        __syncthreads();
+    }
+    const int n_tiles = p.offsets ? first_s[p.experts] : token_tiles((int)p.rows) * p.tiles_c;
+    const int k_steps = ((p.K + 127) / 128 + PAIR_BLOCKS - 1) / PAIR_BLOCKS;
+    const Tail tail = tail_plan(n_tiles, k_steps, pairs, true);
+    constexpr int CHUNKS = PAIR_TOKENS / TAIL_TOKENS, WIDTH = GATED ? 64 : 128;
+    const int t = blockIdx.x / (2 * CHUNKS), rank = blockIdx.x / CHUNKS & 1, c0 = blockIdx.x % CHUNKS * TAIL_TOKENS;
+    if (!tail.split || tail.full + t >= n_tiles) return;
+    TileOrder order = {p, p.offsets ? first_s : nullptr, row_s, band, p.offsets ? expert_of_tile(p, first_s, tail.full + t) : 0};
+    const Tile tile = order.at(tail.full + t);
+    if (c0 >= tile.n_rows) return;
+    Lane L = make_lane<GATED>(p, tile, (int64_t)tile.ct * 2 * WIDTH + rank * WIDTH, c, sx_s - c0);
+    if (c < TAIL_TOKENS) sx_s[c] = c0 + c < tile.n_rows ? p.xs[tile.row0 + c0 + c] : 0.f;
+    __syncthreads();
+    const uint32_t* from = p.pieces + ((size_t)(2 * t * tail.split + rank) * PAIR_TOKENS + c0) * 128 + c;
+    uint32_t v[TAIL_TOKENS];
+#pragma unroll
+    for (int j = 0; j < TAIL_TOKENS; ++j) v[j] = 0;
+    for (int s = 0; s < tail.split; s += 4) {
+        uint32_t u[4][TAIL_TOKENS];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < TAIL_TOKENS; ++j) u[i][j] = __ldcg(from + (size_t)min(s + i, tail.split - 1) * (2 * PAIR_TOKENS * 128) + j * 128);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (s + i < tail.split)
+#pragma unroll
+                for (int j = 0; j < TAIL_TOKENS; ++j) v[j] += u[i][j];
+    }
+    emit<GATED, TAIL_TOKENS>(p, L, c0, v);
 }
 
 // Weights (experts, 1 or 2, channels, K) and a box of 128 rows of 128 bytes; the order of the dimensions interleaves the two
@@ -885,7 +1003,14 @@ int launch_pair(const W8A8Problem& w, Params p, bool dependent, cudaStream_t st)
     const int resident = dev >= 0 && dev < 64 && g_pairs_resident[dev] > 0 ? g_pairs_resident[dev] : sm_count() / 2;
     const int64_t most = ((int64_t)token_tiles((int)w.rows) + (w.offsets ? std::min(w.experts, w.rows) : 0)) * p.tiles_c;
     if (most > 0x7fffffffll) return fail(WUSH_ERR_UNSUPPORTED, "w8a8: too many tiles (%lld)", (long long)most);
-    const int pairs = (int)std::min<int64_t>(most, resident);
+    const int k_steps = (int)(((w.K + 127) / 128 + PAIR_BLOCKS - 1) / PAIR_BLOCKS);
+    // With experts only the device knows the number of tiles; there the second kernel is launched where a cut could pay at all.
+    const bool cut = w.offsets ? k_steps - (k_steps + 1) / 2 > TAIL_STAGES : tail_plan((int)most, k_steps, resident, true).split > 0;
+    const int pairs = cut ? resident : (int)std::min<int64_t>(most, resident);
+    if (!cut) p.pieces = nullptr;
+    // The token tiles of a channel block run at the same time if there are few of them: its weights pass L2 once.
+    // Where more tiles share them the hint costs (8192 x 18944, 2048 rows: 203 -> 212 us); below it pays (333 rows: 82 -> 79).
+    p.weights_once = w.offsets ? w.rows <= PAIR_TOKENS * std::min(w.experts, w.rows) : token_tiles((int)w.rows) <= 4;
     // Band of token tiles whose activations take about a quarter of the L2 (32 MB).
     const int band = (int)std::max<int64_t>(2, std::min<int64_t>(token_tiles((int)w.rows), (32ll << 20) / (PAIR_TOKENS * w.K)));
     cudaLaunchConfig_t cfg = {};
@@ -899,6 +1024,10 @@ int launch_pair(const W8A8Problem& w, Params p, bool dependent, cudaStream_t st)
     cfg.attrs = attr;
     cfg.numAttrs = dependent ? 1 : 0;
     cudaError_t e = cudaLaunchKernelEx(&cfg, w8a8_pair_kernel<GATED>, maps, p, band);
+    if (e == cudaSuccess && cut) {
+        const int64_t rest = w.offsets ? std::min<int64_t>(most, pairs - 1) : most % pairs;
+        e = launch_dependent(w8a8_tail_kernel<GATED>, dim3((unsigned)(rest * 2 * (PAIR_TOKENS / TAIL_TOKENS))), dim3(128), 0, st, p, band, pairs);
+    }
     if (e != cudaSuccess) return fail(WUSH_ERR_CUDA, "w8a8: launch failed: %s", cudaGetErrorString(e));
     return WUSH_OK;
 }
@@ -960,11 +1089,11 @@ int w8a8_take_error(int* word)
     return e == cudaSuccess ? WUSH_OK : fail(WUSH_ERR_CUDA, "device_flag(w8a8): %s", cudaGetErrorString(e));
 }
 
-// Counters, then the slots of the streaming kernel; 0 where the pairs run.
+// Counters, then the slots of the streaming kernel (two per CTA) or of the pair kernel (one per CTA).
 size_t w8a8_workspace_bytes(int64_t rows, int64_t experts)
 {
     const int nt = stream_tokens(rows, experts);
-    return nt ? W8A8_COUNTER_BYTES + (size_t)2 * sm_count() * 128 * nt * sizeof(int32_t) : 0;
+    return W8A8_COUNTER_BYTES + (size_t)sm_count() * 128 * (nt ? 2 * nt : PAIR_TOKENS) * sizeof(int32_t);
 }
 
 int w8a8_launch(const W8A8Problem& w, void* workspace, bool dependent, cudaStream_t st)
@@ -976,9 +1105,9 @@ int w8a8_launch(const W8A8Problem& w, void* workspace, bool dependent, cudaStrea
     p.bf16_out = w.out_dtype == WUSH_BF16;
     p.early = dependent ? 1 : 0;
     const int nt = stream_tokens(w.rows, w.experts);
-    if (nt == 0) return w.gated ? launch_pair<true>(w, p, dependent, st) : launch_pair<false>(w, p, dependent, st);
     p.counters = (int32_t*)workspace;
     p.pieces = (uint32_t*)((uint8_t*)workspace + W8A8_COUNTER_BYTES);
+    if (nt == 0) return w.gated ? launch_pair<true>(w, p, dependent, st) : launch_pair<false>(w, p, dependent, st);
 #define WUSH_STREAM(NT) return w.gated ? launch_stream<NT, true>(w, p, dependent, st) : launch_stream<NT, false>(w, p, dependent, st)
     if (nt == 16) WUSH_STREAM(16);
     if (nt == 32) WUSH_STREAM(32);
@@ -1014,10 +1143,10 @@ int launch_alone(const char* op, const wush::W8A8Problem& p, void* workspace, si
 {
     using namespace wush;
     const size_t need = w8a8_workspace_bytes(p.rows, p.experts);
-    if (need) {
-        if (!workspace || workspace_bytes < need)
-            return fail(WUSH_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, %zu given", op, need, workspace ? workspace_bytes : (size_t)0);
-        WUSH_REQUIRE(aligned16(workspace), "%s: the workspace must be 16-byte aligned", op);
+    if (!workspace || workspace_bytes < need)
+        return fail(WUSH_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, %zu given", op, need, workspace ? workspace_bytes : (size_t)0);
+    WUSH_REQUIRE(aligned16(workspace), "%s: the workspace must be 16-byte aligned", op);
+    if (stream_tokens(p.rows, p.experts)) {                             // the pair kernel has no counters
         cudaError_t e = cudaMemsetAsync(workspace, 0, W8A8_COUNTER_BYTES, st);
         if (e != cudaSuccess) return fail(WUSH_ERR_CUDA, "%s: cudaMemsetAsync: %s", op, cudaGetErrorString(e));
     }
@@ -1106,7 +1235,7 @@ WUSH_API int wush_w8a8_linear(const void* x, int dtype, const int8_t* wq, const 
     if (int e = check_product("w8a8_linear", p)) return e;
     if (M == 0 || N == 0) return WUSH_OK;
     if (int e = ensure_init()) return e;
-    const QuantRows q = {x, dtype, M, K, xq, xs, nullptr, 1, nullptr, w8a8_workspace_bytes(M, 1) ? (int32_t*)workspace : nullptr};
+    const QuantRows q = {x, dtype, M, K, xq, xs, nullptr, 1, nullptr, (int32_t*)workspace};
     if (int e = quant_int8_launch(q, false, (cudaStream_t)stream)) return e;
     return w8a8_launch(p, workspace, true, (cudaStream_t)stream);
 }
@@ -1177,13 +1306,78 @@ WUSH_API int wush_w8a8_expert_ffn(const void* x, int dtype, const void* ids, int
     if (int e = check_product("w8a8_expert_ffn", down)) return e;
     if (int e = ensure_init()) return e;
     cudaStream_t st = (cudaStream_t)stream;
-    const bool counted = w8a8_workspace_bytes(f.R, experts) != 0;       // both products of a block run on the same kernel
-    const QuantRows qx = {x, dtype, tokens, H, xq, xs, pos, (int)k, offsets + experts, counted ? (int32_t*)(base + f.up) : nullptr};
-    const QuantRows qh = {h, WUSH_F32, f.R, I, hq, hs, nullptr, 1, nullptr, counted ? (int32_t*)(base + f.down) : nullptr};
+    const QuantRows qx = {x, dtype, tokens, H, xq, xs, pos, (int)k, offsets + experts, (int32_t*)(base + f.up)};
+    const QuantRows qh = {h, WUSH_F32, f.R, I, hq, hs, nullptr, 1, nullptr, (int32_t*)(base + f.down)};
     if (int e = expert_sort_launch(ids, id_bytes, f.R, (int)experts, pos, offsets, st)) return e;
     if (int e = quant_int8_launch(qx, true, st)) return e;
     if (int e = w8a8_launch(up, base + f.up, true, st)) return e;
     if (int e = quant_int8_launch(qh, true, st)) return e;
     if (int e = w8a8_launch(down, base + f.down, true, st)) return e;
     return expert_combine_launch(base + f.o, dtype, tokens, H, pos, (int)k, weights, y, true, st);
+}
+
+// Host walk of both kernels' division of work, for the test suite.
+namespace {
+int walk_division(int kernel, int tiles, int k_steps, int ctas, int* cover, int* cut)
+{
+    using namespace wush;
+    *cut = 0;
+    if (kernel == 0) {                                   // streaming: ctas CTAs, two slots each
+        std::vector<int> parts(tiles, 0), slots(2 * (size_t)ctas, 0);
+        for (int b = 0; b < ctas; ++b) {
+            const Run run = make_run(tiles, k_steps, b, ctas);
+            int seen = 0;
+            for (int i = 0; i < run.pieces; ++i) {
+                const Piece q = piece_of(run, i);
+                if (q.t < 0 || q.t >= tiles || q.k0 < 0 || q.k0 >= q.k1 || q.k1 > k_steps) return 101;
+                for (int k = q.k0; k < q.k1; ++k) ++cover[(size_t)q.t * k_steps + k];
+                seen += q.k1 - q.k0;
+                if (q.k1 - q.k0 == k_steps) continue;
+                const int first = owner(run, q.t * k_steps), last = owner(run, q.t * k_steps + k_steps - 1);
+                if (b < first || b > last || (b == first) != (q.k0 == 0)) return 102;
+                if (++slots[2 * (size_t)b + (q.k0 == 0)] > 1) return 103;      // a slot holds one piece
+                ++parts[q.t];
+            }
+            if (seen != run.end - run.begin) return 104;
+        }
+        for (int t = 0; t < tiles; ++t)
+            if (parts[t]) {                              // the count that the last CTA waits to see
+                ++*cut;
+                const Run run = make_run(tiles, k_steps, 0, ctas);
+                if (parts[t] != owner(run, t * k_steps + k_steps - 1) - owner(run, t * k_steps) + 1) return 105;
+            }
+        return WUSH_OK;
+    }
+    const Tail tail = tail_plan(tiles, k_steps, ctas, true);
+    std::vector<int> parts(tiles, 0);
+    for (int b = 0; b < ctas; ++b) {
+        int pieces = 0;
+        for (int i = 0;; ++i) {
+            const Work w = work_of(tail, tiles, k_steps, b, ctas, i);
+            if (!w.valid) break;
+            if (w.t < 0 || w.t >= tiles || w.k0 < 0 || w.k0 >= w.k1 || w.k1 > k_steps || w.whole != (w.k1 - w.k0 == k_steps)) return 101;
+            for (int k = w.k0; k < w.k1; ++k) ++cover[(size_t)w.t * k_steps + k];
+            if (w.whole) continue;
+            if (++pieces > 1) return 103;                // a pair has one slot
+            if (b != (w.t - tail.full) * tail.split + parts[w.t]) return 105;  // where the second kernel looks for part parts[t]
+            ++parts[w.t];
+        }
+    }
+    for (int t = 0; t < tiles; ++t) {
+        if (parts[t] && (t < tail.full || parts[t] != tail.split)) return 106;
+        *cut += parts[t] != 0;
+    }
+    return WUSH_OK;
+}
+}  // namespace
+
+WUSH_API int wush_debug_w8a8_cover(int kernel, int tiles, int k_steps, int ctas, int* cover, int* cut)
+{
+    using namespace wush;
+    WUSH_REQUIRE((kernel == 0 || kernel == 1) && tiles >= 0 && k_steps >= 1 && ctas >= 1 && cover && cut, "w8a8_cover: bad argument");
+    try {
+        return walk_division(kernel, tiles, k_steps, ctas, cover, cut);
+    } catch (const std::bad_alloc&) {
+        return fail(WUSH_ERR_UNSUPPORTED, "w8a8_cover: out of host memory");
+    }
 }
