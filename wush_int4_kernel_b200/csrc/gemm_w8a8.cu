@@ -118,7 +118,7 @@ struct Lane {
 // m + 1: the even lane ends with both values of token m, the odd lane with both of token m + 1, so that 16-bit results leave
 // as 4-byte stores (64 bytes per token and warp) and a gated pair meets without another exchange.  Straight-line code, and
 // scales loaded before the first store: with a branch per pair, or with loads that wait for the stores in front of them
-// because they might alias, a warp stalls once per pair (gated, 32 tokens: 1.7 us; as it stands EMIT_US).
+// because they might alias, a warp stalls once per pair (gated, 32 tokens: 1.7 us; as it stands 0.6).
 template <bool GATED, int COUNT>
 __device__ __forceinline__ void emit(const Params& p, const Lane& L, int m0, const uint32_t* v)
 {
@@ -268,13 +268,13 @@ __device__ __forceinline__ void zero_tail(const Params& p, int64_t used, int tid
 // Bound by the bytes of the weights.  One CTA per multiprocessor with a ring of 8 to 12 stages (128 weight rows x 128 bytes
 // each, 190 KB and more in flight), a producer that runs ahead over tile borders and two accumulators, so that the stream
 // does not pause for a tile's end.  Work is the sequence of all stages, tile after tile, cut into one contiguous run per CTA.
-// Runs end at tile borders where that costs no more than FIXUP_STAGES stages of balance; otherwise they are of equal length,
+// Runs end at tile borders where that costs no more than FIXUP_STAGES stages of balance (a CTA's share of 0.4 us each); otherwise they are of equal length,
 // and a tile cut by a border is finished by whichever of its CTAs comes last: every CTA leaves its sums in a slot of the
 // workspace and counts itself in, and the last one adds the slots (int32: in any order the same sum).  Nobody waits.
 // The usual last one is the CTA whose run ends inside the tile: the next CTA began its run with the rest of it.  It looks
 // at the count before its own sums are complete, and where all the others are in it adds their slots to its accumulator
 // and stores nothing (4096 x 24576: 24 tokens 24.9 -> 23.4 us, 64 tokens 29.1 -> 27.2 us).
-constexpr int FIXUP_STAGES = 8;
+template <int NT> constexpr int FIXUP_STAGES = NT <= 32 ? 12 : 28;      // one token: 2048 x 8192 11.0 us uncut, 11.8 cut; 64 tokens: 4096 x 4096 15.9 and 18.0
 
 struct Run {
     int begin, end;              // stages of this CTA
@@ -282,14 +282,14 @@ struct Run {
     int k_steps;
     int pieces;                  // tiles and parts of tiles in the run
 };
-__host__ __device__ inline Run make_run(int tiles, int k_steps, int cta, int ctas)
+__host__ __device__ inline Run make_run(int tiles, int k_steps, int cta, int ctas, int fixup)
 {
     Run r;
     const int total = tiles * k_steps, per = tiles / ctas, more = tiles - per * ctas;
     r.k_steps = k_steps;
     r.size = total / ctas;
     r.longer = total - r.size * ctas;
-    const int whole = (per + (more ? 1 : 0)) * k_steps, even = r.size + (r.longer ? 1 : 0) + FIXUP_STAGES;
+    const int whole = (per + (more ? 1 : 0)) * k_steps, even = r.size + (r.longer ? 1 : 0) + fixup;
     if (whole > even) {          // a CTA without a stage of its own (total < ctas) has an empty run
         r.begin = cta * r.size + min(cta, r.longer);
         r.end = r.begin + r.size + (cta < r.longer ? 1 : 0);
@@ -326,15 +326,28 @@ __device__ __forceinline__ int ld_acquire(const int32_t* p)
     asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
     return v;
 }
-// Adds columns [c0, c0 + 16) of channel c from the slots of CTAs c_first..c_last but `own`.
+// Adds columns [c0, c0 + 16) of channel c from the slots of CTAs c_first..c_last but `own`, four slots at once: one after
+// another they take a trip to L2 each (4096 x 4096, 64 tokens, five CTAs per tile: 21.5 us, 18.0 with this).
 template <int NT>
 __device__ __forceinline__ void add_slots(const Params& p, uint32_t* v, int c0, int c, int c_first, int c_last, int own)
 {
-    for (int k = c_first; k <= c_last; ++k) {
-        if (k == own) continue;
-        const uint32_t* from = p.pieces + (size_t)(2 * k + (k == c_first)) * Stream<NT>::PIECE + c0 * 128 + c;
+    for (int k = c_first; k <= c_last; k += 4) {
 #pragma unroll
-        for (int j = 0; j < 16; ++j) v[j] += __ldcg(from + j * 128);
+        for (int h = 0; h < 16; h += 8) {
+            uint32_t u[4][8];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int at = min(k + i, c_last);
+                const uint32_t* from = p.pieces + (size_t)(2 * at + (at == c_first)) * Stream<NT>::PIECE + (c0 + h) * 128 + c;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) u[i][j] = __ldcg(from + j * 128);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (k + i <= c_last && k + i != own)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) v[h + j] += u[i][j];
+        }
     }
 }
 
@@ -404,7 +417,7 @@ __global__ void __launch_bounds__(THREADS, 1) w8a8_stream_kernel(const __grid_co
     const uint32_t tmem = *tmem_slot;
     const int k_steps = (p.K + 127) / 128;
     const int n_tiles = p.offsets ? first_s[p.experts] : ((int)p.rows + NT - 1) / NT * p.tiles_c;
-    const Run run = make_run(n_tiles, k_steps, blockIdx.x, gridDim.x);
+    const Run run = make_run(n_tiles, k_steps, blockIdx.x, gridDim.x, FIXUP_STAGES<NT>);
     const int e_first = p.offsets ? expert_of_tile(p, first_s, run.begin / k_steps) : 0;
     StreamOrder<NT> order = {p, p.offsets ? first_s : nullptr, row_s, e_first};
     constexpr int WIDTH = GATED ? 64 : 128;
@@ -1063,10 +1076,13 @@ int set_pair()
 
 }  // namespace
 
-// Token columns of the streaming kernel's tiles, 0 for the pair kernel: by the mean number of rows of an expert.
+// Token columns of the streaming kernel's tiles, 0 for the pair kernel: by the rows of an expert.  Routers spread them, so half
+// the mean is added (64 tokens, 4 of 8 experts, 4096 x 3584: 98 us with tiles for the mean of 32, 74 so).  Dense, 8192 x 57344:
+// 64 rows 79 us streamed and 87 in pairs, 65 rows 85 (tiles of 128 columns) and 90, but 4096 x 24576, 100 rows 30.4 and 29.1.
 static int stream_tokens(int64_t rows, int64_t experts)
 {
-    const int64_t groups = std::min(experts, rows), per = groups ? (rows + groups - 1) / groups : 0;
+    const int64_t groups = std::min(experts, rows), mean = groups ? (rows + groups - 1) / groups : 0;
+    const int64_t per = experts > 1 ? mean * 3 / 2 : mean;
     return per <= 16 ? 16 : per <= 32 ? 32 : per <= 64 ? 64 : 0;
 }
 
@@ -1325,7 +1341,7 @@ int walk_division(int kernel, int tiles, int k_steps, int ctas, int* cover, int*
     if (kernel == 0) {                                   // streaming: ctas CTAs, two slots each
         std::vector<int> parts(tiles, 0), slots(2 * (size_t)ctas, 0);
         for (int b = 0; b < ctas; ++b) {
-            const Run run = make_run(tiles, k_steps, b, ctas);
+            const Run run = make_run(tiles, k_steps, b, ctas, FIXUP_STAGES<16>);
             int seen = 0;
             for (int i = 0; i < run.pieces; ++i) {
                 const Piece q = piece_of(run, i);
@@ -1343,7 +1359,7 @@ int walk_division(int kernel, int tiles, int k_steps, int ctas, int* cover, int*
         for (int t = 0; t < tiles; ++t)
             if (parts[t]) {                              // the count that the last CTA waits to see
                 ++*cut;
-                const Run run = make_run(tiles, k_steps, 0, ctas);
+                const Run run = make_run(tiles, k_steps, 0, ctas, FIXUP_STAGES<16>);
                 if (parts[t] != owner(run, t * k_steps + k_steps - 1) - owner(run, t * k_steps) + 1) return 105;
             }
         return WUSH_OK;

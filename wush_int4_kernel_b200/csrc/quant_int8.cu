@@ -226,7 +226,7 @@ __global__ void __launch_bounds__(1024) quant_int8_kernel(const T* __restrict__ 
 }
 
 // Threads per row.  Few rows: a thread for every 16 elements.  Many: as many steps per thread as the registers hold
-// (333 x 28672 bf16: QUANT_US).
+// (333 x 28672 bf16: 9.7 us with half of that, 7.7).
 template <typename T>
 int threads_per_row(int64_t rows, int64_t K)
 {
