@@ -242,7 +242,7 @@ typedef enum { WUSH_BF16 = 0, WUSH_F16 = 1, WUSH_F32 = 2 } wush_dtype;
 int wush_quant_int8(const void* x, int dtype, int64_t rows, int64_t K, int8_t* q, float* s, void* stream);
 
 /* y[m][n] = xs[m] * ws[n] * sum_k xq[m][k] * wq[n][k] (+ bias[n]), exact int32 sums, scales in fp32, one
- * rounding to `out_dtype` (WUSH_F16 or WUSH_BF16).  bias: N fp32 or NULL.
+ * rounding to `out_dtype`.  bias: N fp32 or NULL.
  * Scratch: wush_w8a8_gemm_workspace_bytes(M, 1), contents irrelevant, 16-byte aligned (may be NULL where that
  * is 0); calls that may run at the same time need their own. */
 size_t wush_w8a8_gemm_workspace_bytes(int64_t M, int64_t experts);
@@ -263,7 +263,8 @@ int wush_w8a8_linear(const void* x, int dtype, const int8_t* wq, const float* ws
  *   offsets  (experts + 1) int32: first row of each expert; offsets[experts] = number of entries
  * gather: rows[pos] = x[t]; the R - offsets[experts] rows behind the last entry become zero.
  * combine: y[t] = sum over j of weights[t][j] * rows[pos[t][j]], fp32 sums in ascending j, entries with
- *   pos -1 neither read nor weighted; weights NULL = ones, which is the gradient of gather.
+ *   pos -1 neither read nor weighted; weights NULL = ones, which is the gradient of gather.  `out_dtype`: that of the
+ *   rows, or any of fp32 rows.
  * combine_grad: d_rows[pos] = weights * dy[t] (rows behind the last entry zero), d_weights[t][j] =
  *   <dy[t], rows[pos]> in fp32 (0 where there is no expert).
  * No result depends on an order of execution.  H: any length; rows that are a multiple of 16 bytes at
@@ -274,7 +275,7 @@ int wush_expert_gather(const void* x, int dtype, int64_t tokens, int64_t H, cons
                        const int32_t* offsets, int64_t experts, void* rows, void* stream);
 int wush_expert_gather_quant_int8(const void* x, int dtype, int64_t tokens, int64_t K, const int32_t* pos, int64_t k,
                                   const int32_t* offsets, int64_t experts, int8_t* q, float* s, void* stream);
-int wush_expert_combine(const void* rows, int dtype, int64_t tokens, int64_t H, const int32_t* pos, int64_t k,
+int wush_expert_combine(const void* rows, int dtype, int out_dtype, int64_t tokens, int64_t H, const int32_t* pos, int64_t k,
                         const float* weights, void* y, void* stream);
 int wush_expert_combine_grad(const void* dy, const void* rows, int dtype, int64_t tokens, int64_t H, const int32_t* pos,
                              int64_t k, const int32_t* offsets, int64_t experts, const float* weights, void* d_rows,
@@ -295,8 +296,8 @@ int wush_w8a8_grouped_gated(const int8_t* xq, const float* xs, const int8_t* wq,
 
 /* The whole block: sort, gather + quantise, gated product, quantise, product, weighted sum.
  * x, y: (tokens, H) of `dtype` (WUSH_F16 or WUSH_BF16); weights (tokens, k) fp32; w13q (experts, 2 * I, H),
- * w13s (experts, 2 * I), w2q (experts, H, I), w2s (experts, H).  The experts' outputs are rounded to `dtype`
- * before the weighted sum, which is fp32. */
+ * w13s (experts, 2 * I), w2q (experts, H, I), w2s (experts, H).  The weighted sum is fp32; so are the
+ * experts' outputs that it reads up to 64 MB of them (tokens * k * H * 4 bytes), beyond they are rounded to `dtype`. */
 size_t wush_w8a8_expert_ffn_workspace_bytes(int64_t tokens, int64_t H, int64_t I, int64_t experts, int64_t k);
 int wush_w8a8_expert_ffn(const void* x, int dtype, const void* ids, int id_bytes, const float* weights, const int8_t* w13q,
                          const float* w13s, const int8_t* w2q, const float* w2s, int64_t tokens, int64_t H, int64_t I,

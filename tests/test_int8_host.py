@@ -29,7 +29,7 @@ def test_quant_int8_refusals(lib, args):
 @pytest.mark.parametrize("change", [
     dict(K=40), dict(K=0), dict(K=capi.W8A8_MAX_K + 16), dict(M=-1), dict(N=-1), dict(M=1 << 31), dict(N=1 << 31),
     dict(xq=None), dict(xs=None), dict(wq=None), dict(ws=None), dict(y=None), dict(xq=P + 4), dict(wq=P + 8), dict(xs=P + 2),
-    dict(bias=P + 1), dict(y=P + 2), dict(out=capi.F32), dict(out=9),
+    dict(bias=P + 1), dict(y=P + 2), dict(out=-1), dict(out=9),
 ])
 def test_w8a8_gemm_refusals(lib, change):
     a = dict(xq=P, xs=P, wq=P, ws=P, bias=None, M=4, N=64, K=64, y=P, out=capi.F16) | change
@@ -64,7 +64,7 @@ def test_expert_sort_refusals(lib, change):
 
 def test_expert_entries_limit(lib):
     assert lib.wush_expert_sort(P, 8, 1 << 30, 2, 8, P, P, None) == UNSUPPORTED
-    assert lib.wush_expert_combine(P, capi.BF16, 1 << 30, 64, P, 2, None, P, None) == UNSUPPORTED
+    assert lib.wush_expert_combine(P, capi.BF16, capi.BF16, 1 << 30, 64, P, 2, None, P, None) == UNSUPPORTED
 
 
 @pytest.mark.parametrize("change", [
@@ -76,7 +76,12 @@ def test_expert_moves_refusals(lib, change):
     assert lib.wush_expert_gather_quant_int8(a["x"], a["dt"], a["T"], a["H"], a["pos"], a["k"], a["off"], a["E"], a["out"], P, None) == BAD
     assert lib.wush_expert_combine_grad(a["x"], P, a["dt"], a["T"], a["H"], a["pos"], a["k"], a["off"], a["E"], P, a["out"], P, None) == BAD
     if not {"off", "E"} & set(change):
-        assert lib.wush_expert_combine(a["x"], a["dt"], a["T"], a["H"], a["pos"], a["k"], None, a["out"], None) == BAD
+        assert lib.wush_expert_combine(a["x"], a["dt"], a["dt"], a["T"], a["H"], a["pos"], a["k"], None, a["out"], None) == BAD
+
+
+def test_expert_combine_types(lib):
+    for dt, out in ((capi.BF16, capi.F16), (capi.F16, capi.F32), (capi.F32, 3), (capi.F32, -1)):
+        assert lib.wush_expert_combine(P, dt, out, 4, 32, P, 2, None, P, None) == BAD
 
 
 def test_expert_gather_quant_needs_sixteen(lib):

@@ -48,7 +48,7 @@ SIGNATURES = {
     "wush_expert_sort": (_int, [_vp, _int, _i64, _i64, _i64, _vp, _vp, _vp]),
     "wush_expert_gather": (_int, [_vp, _int, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _vp]),
     "wush_expert_gather_quant_int8": (_int, [_vp, _int, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _vp]),
-    "wush_expert_combine": (_int, [_vp, _int, _i64, _i64, _vp, _i64, _vp, _vp, _vp]),
+    "wush_expert_combine": (_int, [_vp, _int, _int, _i64, _i64, _vp, _i64, _vp, _vp, _vp]),
     "wush_expert_combine_grad": (_int, [_vp, _vp, _int, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp]),
     "wush_w8a8_grouped_gemm": (_int, [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _int, _vp, _sz, _vp]),
     "wush_w8a8_grouped_gated": (_int, [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _vp, _sz, _vp]),

@@ -353,8 +353,9 @@ void* ptr_or_null(const torch::Tensor& t) { return t.defined() ? t.data_ptr() : 
 
 int out_code(torch::ScalarType d, const char* op)
 {
-    TORCH_CHECK(d == torch::kHalf || d == torch::kBFloat16, op, ": out_dtype must be torch.float16 or torch.bfloat16");
-    return d == torch::kHalf ? WUSH_F16 : WUSH_BF16;
+    TORCH_CHECK(d == torch::kHalf || d == torch::kBFloat16 || d == torch::kFloat32, op,
+                ": out_dtype must be torch.float16, torch.bfloat16 or torch.float32");
+    return d == torch::kHalf ? WUSH_F16 : d == torch::kBFloat16 ? WUSH_BF16 : WUSH_F32;
 }
 
 torch::Tensor w8a8_gemm(const torch::Tensor& xq, const torch::Tensor& xs, const torch::Tensor& wq, const torch::Tensor& ws, const c10::optional<torch::Tensor>& bias,
@@ -476,7 +477,8 @@ void check_weights(const torch::Tensor& w, const torch::Tensor& pos, const torch
     TORCH_CHECK(w.sizes() == pos.sizes(), op, ": weights must be (tokens, k)");
 }
 
-torch::Tensor expert_combine(const torch::Tensor& rows, const torch::Tensor& pos, const c10::optional<torch::Tensor>& weights)
+torch::Tensor expert_combine(const torch::Tensor& rows, const torch::Tensor& pos, const c10::optional<torch::Tensor>& weights,
+                             c10::optional<torch::ScalarType> out_dtype)
 {
     const char* op = "expert_combine";
     check_on(rows, rows, op, "rows");
@@ -486,9 +488,12 @@ torch::Tensor expert_combine(const torch::Tensor& rows, const torch::Tensor& pos
     TORCH_CHECK(pos.dim() == 2 && pos.size(1) >= 1, op, ": pos must be (tokens, k)");
     TORCH_CHECK(rows.dim() == 2 && rows.size(0) == pos.numel() && rows.size(1) >= 1, op, ": rows must be (tokens * k, H)");
     if (weights.has_value()) check_weights(*weights, pos, rows, op);
+    const torch::ScalarType out = out_dtype.value_or(rows.scalar_type());
+    TORCH_CHECK(out == rows.scalar_type() || dt == WUSH_F32, op, ": out_dtype must be the type of rows unless that is fp32");
+    const int code = out_code(out, op);
     const at::cuda::OptionalCUDAGuard guard(rows.device());
-    auto y = new_like({pos.size(0), rows.size(1)}, rows.scalar_type(), rows);
-    check_status(wush_expert_combine(rows.data_ptr(), dt, pos.size(0), rows.size(1), pos.data_ptr<int32_t>(), pos.size(1),
+    auto y = new_like({pos.size(0), rows.size(1)}, out, rows);
+    check_status(wush_expert_combine(rows.data_ptr(), dt, code, pos.size(0), rows.size(1), pos.data_ptr<int32_t>(), pos.size(1),
                                      weights.has_value() ? weights->data_ptr<float>() : nullptr, y.data_ptr(), stream_of(rows)),
                  op);
     return y;
@@ -647,7 +652,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
     m.def("expert_gather_quant_int8", &expert_gather_quant_int8, "quant_int8 of x, then expert_gather of codes and scales", py::arg("x"),
           py::arg("pos"), py::arg("offsets"));
     m.def("expert_combine", &expert_combine, "y[t] = sum_j weights[t, j] * rows[pos[t, j]] (weights None: ones)", py::arg("rows"),
-          py::arg("pos"), py::arg("weights") = py::none());
+          py::arg("pos"), py::arg("weights") = py::none(), py::arg("out_dtype") = py::none());
     m.def("expert_combine_grad", &expert_combine_grad, "gradients of expert_combine: (d_rows, d_weights)", py::arg("dy"),
           py::arg("rows"), py::arg("pos"), py::arg("offsets"), py::arg("weights"));
     m.def("w8a8_grouped_gemm", &w8a8_grouped_gemm, "w8a8_gemm of each expert's rows with its weights", py::arg("xq"), py::arg("xs"),

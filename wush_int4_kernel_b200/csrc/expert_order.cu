@@ -284,10 +284,10 @@ struct Entries {
     }
 };
 
-template <typename T, int N, int AT>
+template <typename T, typename O, int N, int AT>
 __global__ void __launch_bounds__(256, AT <= 4 ? 4 : 3) expert_combine_kernel(const Pack<T, N>* __restrict__ rows, int64_t tokens, int n_vec,
                                                              const int32_t* __restrict__ pos, int k,
-                                                             const float* __restrict__ weights, Pack<T, N>* __restrict__ y)
+                                                             const float* __restrict__ weights, Pack<O, N>* __restrict__ y)
 {
     const int64_t t = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
     Entries<T, N, AT> first;
@@ -312,9 +312,9 @@ __global__ void __launch_bounds__(256, AT <= 4 ? 4 : 3) expert_combine_kernel(co
 #pragma unroll
         for (int u = 0; u < U; ++u)
             if (v + u * (int)blockDim.x < n_vec) {
-                Pack<T, N> o;
+                Pack<O, N> o;
 #pragma unroll
-                for (int i = 0; i < N; ++i) o.v[i] = from_f32<T>(acc[u][i]);
+                for (int i = 0; i < N; ++i) o.v[i] = from_f32<O>(acc[u][i]);
                 y[t * n_vec + v + u * (int)blockDim.x] = o;
             }
     }
@@ -445,27 +445,27 @@ int launch_gather(Pack<T, N>, const void* x, int64_t tokens, int64_t H, const in
                                                                                         n_used, (Pack<T, N>*)rows);
     return check_launch("expert_gather");
 }
-template <typename T, int N, int AT>
+template <typename T, typename O, int N, int AT>
 int launch_combine_at(const void* rows, int64_t tokens, int64_t H, const int32_t* pos, int k, const float* weights, void* y,
                       bool dependent, cudaStream_t st)
 {
     const int n_vec = (int)(H / N), tx = threads_along(n_vec, steps_at_once<T, N>()), ty = 256 / tx;
     const dim3 grid((unsigned)((tokens + ty - 1) / ty)), block(tx, ty);
     if (dependent) {
-        cudaError_t e = launch_dependent(expert_combine_kernel<T, N, AT>, grid, block, 0, st, (const Pack<T, N>*)rows, tokens, n_vec, pos, k,
-                                         weights, (Pack<T, N>*)y);
+        cudaError_t e = launch_dependent(expert_combine_kernel<T, O, N, AT>, grid, block, 0, st, (const Pack<T, N>*)rows, tokens, n_vec, pos, k,
+                                         weights, (Pack<O, N>*)y);
         if (e != cudaSuccess) return fail(WUSH_ERR_CUDA, "expert_combine: launch failed: %s", cudaGetErrorString(e));
         return WUSH_OK;
     }
-    expert_combine_kernel<T, N, AT><<<grid, block, 0, st>>>((const Pack<T, N>*)rows, tokens, n_vec, pos, k, weights, (Pack<T, N>*)y);
+    expert_combine_kernel<T, O, N, AT><<<grid, block, 0, st>>>((const Pack<T, N>*)rows, tokens, n_vec, pos, k, weights, (Pack<O, N>*)y);
     return check_launch("expert_combine");
 }
-template <typename T, int N>
+template <typename O, typename T, int N>
 int launch_combine(Pack<T, N>, const void* rows, int64_t tokens, int64_t H, const int32_t* pos, int k, const float* weights, void* y,
                    bool dependent, cudaStream_t st)
 {
     return with_count(k, [&](auto at) {
-        return launch_combine_at<T, N, decltype(at)::value>(rows, tokens, H, pos, k, weights, y, dependent, st);
+        return launch_combine_at<T, O, N, decltype(at)::value>(rows, tokens, H, pos, k, weights, y, dependent, st);
     });
 }
 template <typename T, int N, int AT>
@@ -514,11 +514,18 @@ int expert_sort_launch(const void* ids, int id_bytes, int64_t n, int n_experts, 
     return launch_sort<int32_t>((const int32_t*)ids, n, n_experts, pos, offsets, st);
 }
 
-int expert_combine_launch(const void* rows, int dtype, int64_t tokens, int64_t H, const int32_t* pos, int k, const float* weights,
-                          void* y, bool dependent, cudaStream_t st)
+int expert_combine_launch(const void* rows, int dtype, int out_dtype, int64_t tokens, int64_t H, const int32_t* pos, int k,
+                          const float* weights, void* y, bool dependent, cudaStream_t st)
 {
-    return with_type(dtype, common_align(dtype, H, rows, y, y),
-                     [&](auto p) { return launch_combine(p, rows, tokens, H, pos, k, weights, y, dependent, st); });
+    if (dtype == out_dtype)
+        return with_type(dtype, common_align(dtype, H, rows, y, y), [&](auto p) {
+            return launch_combine<std::decay_t<decltype(p.v[0])>>(p, rows, tokens, H, pos, k, weights, y, dependent, st);
+        });
+    const int align = common_align(WUSH_F32, H, rows, (const void*)((uintptr_t)y * 2), rows);      // y in halves of the rows' packs
+    return with_pack<float>(align, [&](auto p) {
+        if (out_dtype == WUSH_BF16) return launch_combine<__nv_bfloat16>(p, rows, tokens, H, pos, k, weights, y, dependent, st);
+        return launch_combine<__half>(p, rows, tokens, H, pos, k, weights, y, dependent, st);
+    });
 }
 
 }  // namespace wush
@@ -552,18 +559,20 @@ WUSH_API int wush_expert_gather(const void* x, int dtype, int64_t tokens, int64_
     });
 }
 
-WUSH_API int wush_expert_combine(const void* rows, int dtype, int64_t tokens, int64_t H, const int32_t* pos, int64_t k,
+WUSH_API int wush_expert_combine(const void* rows, int dtype, int out_dtype, int64_t tokens, int64_t H, const int32_t* pos, int64_t k,
                                  const float* weights, void* y, void* stream)
 {
     using namespace wush;
     if (int e = check_moves("expert_combine", dtype, tokens, H)) return e;
     if (int e = check_entries("expert_combine", tokens, k, 1)) return e;
+    WUSH_REQUIRE(out_dtype == dtype || (dtype == WUSH_F32 && out_dtype >= WUSH_BF16 && out_dtype <= WUSH_F32),
+                 "expert_combine: the result has the type of the rows, or any of fp32 rows");
     if (tokens == 0) return WUSH_OK;
     WUSH_REQUIRE(rows && pos && y, "expert_combine: null pointer");
-    WUSH_REQUIRE(element_aligned(dtype, rows) && element_aligned(dtype, y) && aligned4(pos) && aligned4(weights),
+    WUSH_REQUIRE(element_aligned(dtype, rows) && element_aligned(out_dtype, y) && aligned4(pos) && aligned4(weights),
                  "expert_combine: misaligned pointer");
     if (int e = ensure_init()) return e;
-    return expert_combine_launch(rows, dtype, tokens, H, pos, (int)k, weights, y, false, (cudaStream_t)stream);
+    return expert_combine_launch(rows, dtype, out_dtype, tokens, H, pos, (int)k, weights, y, false, (cudaStream_t)stream);
 }
 
 WUSH_API int wush_expert_combine_grad(const void* dy, const void* rows, int dtype, int64_t tokens, int64_t H, const int32_t* pos, int64_t k,

@@ -36,7 +36,7 @@ struct QuantRows {
 };
 int quant_int8_launch(const QuantRows& a, bool dependent, cudaStream_t st);
 int expert_sort_launch(const void* ids, int id_bytes, int64_t n, int n_experts, int32_t* pos, int32_t* offsets, cudaStream_t st);
-int expert_combine_launch(const void* rows, int dtype, int64_t tokens, int64_t H, const int32_t* pos, int k, const float* weights,
+int expert_combine_launch(const void* rows, int dtype, int out_dtype, int64_t tokens, int64_t H, const int32_t* pos, int k, const float* weights,
                           void* y, bool dependent, cudaStream_t st);
 
 struct W8A8Problem {

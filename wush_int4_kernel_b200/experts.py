@@ -102,8 +102,9 @@ class W8A8Experts:
         xq, xs = route.gather_quant_int8(x)
         h = ops.w8a8_grouped_gated(xq, xs, self.w13q, self.w13s, route.offsets)
         hq, hs = ops.quant_int8(h)
-        o = ops.w8a8_grouped_gemm(hq, hs, self.w2q, self.w2s, route.offsets, x.dtype)
-        return ops.expert_combine(o, route.pos, weights)
+        fp32 = 4 * ids.numel() * x.shape[1] <= 64 << 20           # what the block keeps in fp32 before the weighted sum
+        o = ops.w8a8_grouped_gemm(hq, hs, self.w2q, self.w2s, route.offsets, torch.float32 if fp32 else x.dtype)
+        return ops.expert_combine(o, route.pos, weights, x.dtype)
 
     def to(self, device) -> "W8A8Experts":
         return W8A8Experts(*(t.to(device) for t in (self.w13q, self.w13s, self.w2q, self.w2s)))
