@@ -446,8 +446,9 @@ def test_grouped_gemm(C, sizes, tail, N, K):
 @pytest.mark.parametrize("inner,K", [(64, 128), (500, 272), (37, 1040), (1024, 2048)])
 @pytest.mark.parametrize("sizes,tail", SIZES)
 def test_grouped_gated(C, sizes, tail, inner, K):
-    """g and u carry 3 u each; silu has a relative condition of at most 1 + |g|; expf, the sum, the quotient and the last
-    product add 4 + 1 + 4 + 1 of u; beyond |g| = 80 the exponential leaves the range of fp32 and 1e-30 |u| covers the rest."""
+    """g and u carry 3 u each; silu has a relative condition of at most 1 + |g|; __expf (2 + 1.173 |g| units in the last place,
+    of 2 u each), the sum, the quotient and the last product add 4 + 2.4 |g| + 1 + 4 + 1 of u; beyond |g| = 80 the exponential
+    leaves the range of fp32 and 1e-30 |u| covers the rest."""
     xq, xs, wq, ws, offsets = grouped_case(sizes, tail, 2 * inner, K, gen(sum(sizes) + inner + K))
     h = C.w8a8_grouped_gated(xq, xs, wq, ws, offsets)
     assert h.shape == (xq.shape[0], inner) and h.dtype == torch.float32 and not h[sum(sizes):].any()
@@ -455,7 +456,7 @@ def test_grouped_gated(C, sizes, tail, inner, K):
     for i, n in enumerate(sizes):
         g, u = product64(xq[a:a + n], xs[a:a + n], wq[i], ws[i]).chunk(2, dim=-1)
         want = g * torch.sigmoid(g) * u
-        within(h[a:a + n], want, want.abs() * (3 * (1 + g.abs()) + 3 + 10 + 2) * U + 1e-30 * (1 + u.abs()))
+        within(h[a:a + n], want, want.abs() * (5.4 * g.abs() + 3 + 3 + 10 + 2) * U + 1e-30 * (1 + u.abs()))
         a += n
 
 
@@ -473,7 +474,7 @@ def test_grouped_long_k(C, sizes, tail):
         within(y[a:a + n], want, want.abs() * (e(torch.float16) + 4 * U) + TINY16)
         g, u = want.chunk(2, dim=-1)
         want = g * torch.sigmoid(g) * u
-        within(h[a:a + n], want, want.abs() * (3 * (1 + g.abs()) + 3 + 10 + 2) * U + 1e-30 * (1 + u.abs()))
+        within(h[a:a + n], want, want.abs() * (5.4 * g.abs() + 3 + 3 + 10 + 2) * U + 1e-30 * (1 + u.abs()))
         a += n
 
 

@@ -155,11 +155,46 @@ __global__ void __launch_bounds__(SORT_THREADS) expert_sort_kernel(const Id* __r
     if constexpr (CTAS > 1) cluster_barrier();      // no CTA leaves while its totals may be read
 }
 
+// A few entries (decode): every entry counts the entries in front of it, every expert the entries of smaller ones; ids are
+// compared four at a time from shared memory.  8 entries of 64 experts: 1.6 us against 3.2 of the counting sort, 64 of 64:
+// 2.2; 192 of 32: 3.4 against 3.6, 256 of 128: 6.6 against 4.3.
+constexpr int RANK_MAX = 64;
+template <typename Id>
+__global__ void __launch_bounds__(512) expert_rank_kernel(const Id* __restrict__ ids, int n, int E, int32_t* __restrict__ pos,
+                                                          int32_t* __restrict__ offsets)
+{
+    __shared__ alignas(16) int32_t id_s[RANK_MAX];
+    pdl_wait();
+    pdl_launch_dependents();
+    const int n4 = (n + 3) / 4;
+    for (int i = threadIdx.x; i < 4 * n4; i += blockDim.x) {
+        const int e = expert_of(ids, i, n, E);
+        id_s[i] = e < 0 ? E : e;                    // E: no expert
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i <= n + E; i += blockDim.x) {
+        const bool entry = i < n;
+        const int me = entry ? id_s[i] : i - n, before = entry ? i : 0;
+        int below = 0;
+        for (int j = 0; j < n4; ++j) {
+            const int4 o = reinterpret_cast<const int4*>(id_s)[j];
+            below += (o.x < me || (o.x == me && 4 * j < before)) + (o.y < me || (o.y == me && 4 * j + 1 < before)) +
+                     (o.z < me || (o.z == me && 4 * j + 2 < before)) + (o.w < me || (o.w == me && 4 * j + 3 < before));
+        }
+        if (entry) pos[i] = me < E ? below : -1;
+        else offsets[me] = below;
+    }
+}
+
 size_t sort_smem_bytes(int E) { return (size_t)(SORT_WARPS + 1) * E * sizeof(int32_t); }
 
 template <typename Id>
 int launch_sort(const Id* ids, int64_t n, int E, int32_t* pos, int32_t* offsets, cudaStream_t st)
 {
+    if (n <= RANK_MAX) {
+        expert_rank_kernel<Id><<<1, 512, 0, st>>>(ids, (int)n, E, pos, offsets);
+        return check_launch("expert_sort");
+    }
     const size_t smem = sort_smem_bytes(E);
     if (n <= 2048) {                                // 2048 entries: 5.5 us in one CTA, 7 in a cluster; 4096: 7.5 and 7
         expert_sort_kernel<Id, 1><<<1, SORT_THREADS, smem, st>>>(ids, n, E, pos, offsets);
