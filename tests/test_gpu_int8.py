@@ -496,6 +496,13 @@ def test_grouped_offsets_outside_the_rows_are_cut(C):
     xq, xs, wq, ws, _ = grouped_case([20, 30], 0, 64, 128, gen(8))
     y = C.w8a8_grouped_gemm(xq, xs, wq, ws, torch.tensor([-7, 20, 5000], dtype=torch.int32, device="cuda"))
     assert torch.equal(y, C.w8a8_grouped_gemm(xq, xs, wq, ws, torch.tensor([0, 20, 50], dtype=torch.int32, device="cuda")))
+    # descending ones: every row belongs to at most one expert, the first that reaches it
+    for bad, good in (([0, 50, 20, 50], [0, 50, 50, 50]), ([30, 10, 50, 0], [30, 30, 50, 50]), ([50, 0, 0, 0], [50] * 4)):
+        wq3, ws3 = torch.cat((wq, wq[:1])), torch.cat((ws, ws[:1]))
+        as_int = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+        y, want = (C.w8a8_grouped_gemm(xq, xs, wq3, ws3, as_int(v)) for v in (bad, good))
+        a, b = good[0], good[-1]
+        assert torch.equal(y[a:b], want[a:b])
     pos = torch.tensor([[0, 99], [-5, 1 << 30]], dtype=torch.int32, device="cuda")
     x = randn(2, 128, g=gen(1), dtype=torch.bfloat16)
     rows = C.expert_gather(x, pos, torch.tensor([0, 1], dtype=torch.int32, device="cuda"))
@@ -549,6 +556,47 @@ def test_expert_block(C, T, H, inner, E, k, drop, dtype):
     rounded = e(dtype) if 4 * T * k * H > 64 << 20 else 0.0               # the outputs of the experts, where they leave fp32
     bound = terms.abs().sum(1) * (rounded + (k + 4) * U) + terms.sum(1).abs() * e(dtype) * 1.01 + TINY16 * (k + 1)
     within(y, terms.sum(1), bound)
+
+
+def test_same_expert_twice_and_no_token(C):
+    """A token that names one expert several times counts as often; a block without tokens has no rows."""
+    from wush_int4_kernel_b200.experts import ExpertRoute, W8A8Experts
+    g = gen(21)
+    E, H, inner, T = 4, 64, 32, 50
+    block = W8A8Experts.from_weights(randn(E, 2 * inner, H, g=g) * H ** -0.5, randn(E, H, inner, g=g) * inner ** -0.5)
+    x = randn(T, H, g=g, dtype=torch.bfloat16)
+    ids = torch.randint(0, E, (T, 1), generator=g, device="cuda").expand(T, 3)
+    w = torch.rand(T, 3, generator=g, device="cuda")
+    y, once = block(x, ids, w), block(x, ids[:, :1], w.sum(1, keepdim=True))
+    # the same term three times, summed in fp32 in three steps or one, then one rounding each
+    assert ((y.double() - once.double()).abs() <= once.double().abs() * (2 * e(torch.bfloat16) + 8 * U) + 1e-30).all()
+    route = ExpertRoute.sort(ids, E)
+    assert torch.equal(route.pos.sort(dim=0)[0].view(-1).sort()[0], torch.arange(3 * T, device="cuda", dtype=torch.int32))
+    none = block(x[:0], ids[:0], w[:0])
+    assert none.shape == (0, H) and none.dtype == torch.bfloat16
+    wide = randn(T, 2 * H, g=g, dtype=torch.bfloat16)[:, :H]               # rows with a stride: copied
+    assert torch.equal(block(wide, ids, w), block(wide.contiguous(), ids, w))
+
+
+def test_a_large_block_in_a_graph(C):
+    """The other kernels of the chain (sort in a cluster, CTA pairs, tiles cut along K) captured, replayed on new inputs."""
+    from wush_int4_kernel_b200.experts import W8A8Experts
+    g = gen(31)
+    E, H, inner, T, k = 8, 512, 6160, 900, 4
+    block = W8A8Experts.from_weights(randn(E, 2 * inner, H, g=g, dtype=torch.bfloat16) * H ** -0.5,
+                                     randn(E, H, inner, g=g, dtype=torch.bfloat16) * inner ** -0.5)
+    held = [randn(T, H, g=g, dtype=torch.float16), ids_of(T, k, E, g), torch.softmax(randn(T, k, g=g), -1)]
+    block(*held)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = block(*held)
+    for seed in (1, 2):
+        s = gen(seed)
+        new = [randn(T, H, g=s, dtype=torch.float16), ids_of(T, k, E, s), torch.softmax(randn(T, k, g=s), -1)]
+        for a, b in zip(held, new):
+            a.copy_(b)
+        graph.replay()
+        assert torch.equal(out, block(*new)) and torch.equal(out, block.by_operators(*new))
 
 
 def test_a_step_of_a_block_with_both_widths(C):

@@ -102,7 +102,7 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* r)
         : "r"(taddr)
         : "memory");
 }
-// First row of expert e.  Offsets come from the caller: kept inside the rows, so that a bad one reads nothing out of range.
+// First row of expert e, kept inside the rows: offsets come from the caller (make_table also keeps them ascending).
 __device__ __forceinline__ int first_row(const Params& p, int e) { return max(0, min(__ldcg(p.offsets + e), (int)p.rows)); }
 
 // What a thread of the epilogue needs to turn the sums of its channel into results.
@@ -225,7 +225,7 @@ __device__ __forceinline__ void make_table(const Params& p, int32_t* first, int3
 {
     constexpr int AT_ONCE = 4;                           // 128 experts at once: latency is all that this costs
     const int lane = threadIdx.x & 31;
-    int before = 0;
+    int before = 0, top = 0;
     for (int e0 = 0; e0 < p.experts; e0 += 32 * AT_ONCE) {
         int a[AT_ONCE], b[AT_ONCE], scan[AT_ONCE], tiles[AT_ONCE];
 #pragma unroll
@@ -233,6 +233,20 @@ __device__ __forceinline__ void make_table(const Params& p, int32_t* first, int3
             const int e = e0 + 32 * i + lane;
             a[i] = e < p.experts ? first_row(p, e) : 0;
             b[i] = e < p.experts ? first_row(p, e + 1) : 0;
+        }
+        // Running maximum: bad offsets then give no more tiles than the rows have, and none outside them.
+#pragma unroll
+        for (int d = 1; d < 32; d *= 2)
+#pragma unroll
+            for (int i = 0; i < AT_ONCE; ++i) {
+                const int up = __shfl_up_sync(0xffffffffu, a[i], d);
+                if (lane >= d) a[i] = max(a[i], up);
+            }
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; ++i) {
+            a[i] = max(a[i], top);
+            b[i] = max(a[i], b[i]);
+            top = __shfl_sync(0xffffffffu, a[i], 31);
         }
 #pragma unroll
         for (int i = 0; i < AT_ONCE; ++i) scan[i] = tiles[i] = b[i] > a[i] ? tiles_of(b[i] - a[i]) * p.tiles_c : 0;

@@ -90,9 +90,9 @@ class W8A8Experts:
         return self.w13q.shape[0]
 
     def __call__(self, x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor) -> torch.Tensor:
-        lead, k = x.shape[:-1], ids.shape[-1]
-        y = _ops().w8a8_expert_ffn(x.reshape(-1, x.shape[-1]), ids.reshape(-1, k), weights.reshape(-1, k), self.w13q, self.w13s,
-                                   self.w2q, self.w2s)
+        lead = x.shape[:-1]
+        x2, ids2, w2 = (t.reshape(-1, t.shape[-1]).contiguous() for t in (x, ids, weights))
+        y = _ops().w8a8_expert_ffn(x2, ids2, w2, self.w13q, self.w13s, self.w2q, self.w2s)
         return y.reshape(*lead, x.shape[-1])
 
     def by_operators(self, x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor) -> torch.Tensor:
