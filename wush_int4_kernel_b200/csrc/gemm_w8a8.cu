@@ -627,7 +627,7 @@ __device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t cluster_add
 
 struct PairMaps {
     CUtensorMap w;
-    CUtensorMap x[3];            // boxes of 32, 64, 128 token rows
+    CUtensorMap x[4];            // boxes of 32, 64, 96, 128 token rows
 };
 
 __device__ __forceinline__ void tma_load_4d_pair(void* dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int c2, int c3,
@@ -786,8 +786,8 @@ w8a8_pair_kernel(const __grid_constant__ PairMaps maps, const Params p, int band
                 if (!w.valid) break;
                 const Tile tile = order.at(w.t);
                 const int half = tile.nt / 2, c0 = tile.ct * 2 * WIDTH + (int)rank * WIDTH;
-                const int m = half <= 32 ? 0 : half <= 64 ? 1 : 2, row = (int)tile.row0 + (int)rank * half;
-                const uint32_t bytes = 2 * (A_BYTES + (32 << m) * 128);          // of both CTAs
+                const int m = (half + 31) / 32 - 1, row = (int)tile.row0 + (int)rank * half;
+                const uint32_t bytes = 2 * (A_BYTES + (m + 1) * 32 * 128);          // of both CTAs
                 const CUtensorMap* mx = &maps.x[m];
                 for (int ks = w.k0; ks < w.k1; ++ks) {
                     if (!tc::mbar_wait(&empty[slot], phase ^ 1)) { ok = false; break; }
@@ -1046,8 +1046,8 @@ int launch_pair(const W8A8Problem& w, Params p, bool dependent, cudaStream_t st)
 {
     PairMaps maps;
     if (int e = make_weight_map(&maps.w, w)) return e;
-    for (int i = 0; i < 3; ++i)
-        if (int e = make_token_map(&maps.x[i], w, 32 << i)) return e;
+    for (int i = 0; i < 4; ++i)
+        if (int e = make_token_map(&maps.x[i], w, 32 * (i + 1))) return e;
     p.tiles_c = (int)((w.N + (GATED ? 127 : 255)) / (GATED ? 128 : 256));
     int dev = 0;
     cudaGetDevice(&dev);
