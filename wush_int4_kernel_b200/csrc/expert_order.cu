@@ -363,7 +363,7 @@ __global__ void __launch_bounds__(256, AT <= 4 || steps_at_once<T, N>() > 1 ? 4 
                                                                   const int32_t* __restrict__ n_used, Pack<T, N>* __restrict__ d_rows,
                                                                   float* __restrict__ d_w)
 {
-    constexpr int U = AT <= 4 ? steps_at_once<T, N>() : (steps_at_once<T, N>() + 1) / 2;
+    constexpr int U = steps_at_once<T, N>();
     __shared__ float part[AT][8];
     pdl_wait();
     pdl_launch_dependents();
