@@ -50,6 +50,22 @@ template <int NT> struct Stream {
     static constexpr int PIECE = 128 * NT;                           // sums of a tile
 };
 
+// n / d for n < 2^31 by a multiplication (Granlund and Montgomery 1994): a division is a hundred cycles and more, and at the
+// start of a launch nothing covers it.
+struct Divisor {
+    uint32_t d, mul, shift;
+};
+__host__ __device__ inline Divisor make_divisor(uint32_t d)
+{
+    uint32_t shift = 0;
+    while ((1ull << shift) < d) ++shift;
+    return {d, (uint32_t)((1ull << 32) * ((1ull << shift) - d) / d + 1), shift};
+}
+__host__ __device__ inline int divide(int n, const Divisor& v)
+{
+    return (int)(((uint32_t)(((uint64_t)(uint32_t)n * v.mul) >> 32) + (uint32_t)n) >> v.shift);
+}
+
 struct Params {
     const float* xs;
     const float* ws;
@@ -62,6 +78,7 @@ struct Params {
     int early;                   // weights (and offsets) may be read before the kernel in front has finished
     int32_t* counters;           // one per CTA, zero
     uint32_t* pieces;            // two per CTA
+    Divisor steps, ctas;         // streaming kernel: stages of a tile, CTAs of the launch
     int weights_once;            // pair kernel: what reads a weight does so at about the same time
 };
 
@@ -309,25 +326,28 @@ template <int NT> constexpr int FIXUP_STAGES = NT <= 32 ? 12 : 28;      // one t
 struct Run {
     int begin, end;              // stages of this CTA
     int size, longer;            // a split: every CTA has `size` stages, the first `longer` of them one more
-    int k_steps;
+    int k_steps, first;          // stages of a tile; tile of the first stage
     int pieces;                  // tiles and parts of tiles in the run
 };
-__host__ __device__ inline Run make_run(int tiles, int k_steps, int cta, int ctas, int fixup)
+__host__ __device__ inline Run make_run(int tiles, const Divisor& steps, int cta, const Divisor& ctas, int fixup)
 {
     Run r;
-    const int total = tiles * k_steps, per = tiles / ctas, more = tiles - per * ctas;
+    const int k_steps = (int)steps.d, n = (int)ctas.d, total = tiles * k_steps, per = divide(tiles, ctas), more = tiles - per * n;
     r.k_steps = k_steps;
-    r.size = total / ctas;
-    r.longer = total - r.size * ctas;
+    r.size = divide(total, ctas);
+    r.longer = total - r.size * n;
     const int whole = (per + (more ? 1 : 0)) * k_steps, even = r.size + (r.longer ? 1 : 0) + fixup;
     if (whole > even) {          // a CTA without a stage of its own (total < ctas) has an empty run
         r.begin = cta * r.size + min(cta, r.longer);
         r.end = r.begin + r.size + (cta < r.longer ? 1 : 0);
+        r.first = divide(r.begin, steps);
+        r.pieces = r.end > r.begin ? divide(r.end - 1, steps) - r.first + 1 : 0;
     } else {
-        r.begin = (cta * per + min(cta, more)) * k_steps;
-        r.end = r.begin + (per + (cta < more ? 1 : 0)) * k_steps;
+        r.first = cta * per + min(cta, more);
+        r.pieces = per + (cta < more ? 1 : 0);
+        r.begin = r.first * k_steps;
+        r.end = r.begin + r.pieces * k_steps;
     }
-    r.pieces = r.end > r.begin ? (r.end - 1) / k_steps - r.begin / k_steps + 1 : 0;
     return r;
 }
 // Piece i of a run: stages [k0, k1) of tile t.
@@ -337,7 +357,7 @@ struct Piece {
 __host__ __device__ inline Piece piece_of(const Run& r, int i)
 {
     Piece q;
-    q.t = r.begin / r.k_steps + i;
+    q.t = r.first + i;
     const int start = q.t * r.k_steps;
     q.k0 = max(0, r.begin - start);
     q.k1 = min(r.k_steps, r.end - start);
@@ -445,10 +465,10 @@ __global__ void __launch_bounds__(THREADS, 1) w8a8_stream_kernel(const __grid_co
     __syncthreads();
     tc::tc_fence_after();
     const uint32_t tmem = *tmem_slot;
-    const int k_steps = (p.K + 127) / 128;
+    const int k_steps = (int)p.steps.d;
     const int n_tiles = p.offsets ? first_s[p.experts] : ((int)p.rows + NT - 1) / NT * p.tiles_c;
-    const Run run = make_run(n_tiles, k_steps, blockIdx.x, gridDim.x, FIXUP_STAGES<NT>);
-    const int e_first = p.offsets ? expert_of_tile(p, first_s, run.begin / k_steps) : 0;
+    const Run run = make_run(n_tiles, p.steps, blockIdx.x, p.ctas, FIXUP_STAGES<NT>);
+    const int e_first = p.offsets ? expert_of_tile(p, first_s, run.first) : 0;
     StreamOrder<NT> order = {p, p.offsets ? first_s : nullptr, row_s, e_first};
     constexpr int WIDTH = GATED ? 64 : 128;
 
@@ -1014,8 +1034,10 @@ int launch_stream(const W8A8Problem& w, Params p, bool dependent, cudaStream_t s
     p.tiles_c = (int)((w.N + (GATED ? 63 : 127)) / (GATED ? 64 : 128));
     const int64_t most = stream_tiles(w, NT);
     if (most * ((w.K + 127) / 128) > 0x7fffffffll) return fail(WUSH_ERR_UNSUPPORTED, "w8a8: too many tiles (%lld)", (long long)most);
+    p.steps = make_divisor((uint32_t)((w.K + 127) / 128));
+    p.ctas = make_divisor((uint32_t)sm_count());
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)sm_count());
+    cfg.gridDim = dim3(p.ctas.d);
     cfg.blockDim = dim3(THREADS);
     cfg.dynamicSmemBytes = Stream<NT>::SMEM;
     cfg.stream = st;
@@ -1384,9 +1406,10 @@ int walk_division(int kernel, int tiles, int k_steps, int ctas, int* cover, int*
     using namespace wush;
     *cut = 0;
     if (kernel == 0) {                                   // streaming: ctas CTAs, two slots each
+        const Divisor steps = make_divisor(k_steps), n = make_divisor(ctas);
         std::vector<int> parts(tiles, 0), slots(2 * (size_t)ctas, 0);
         for (int b = 0; b < ctas; ++b) {
-            const Run run = make_run(tiles, k_steps, b, ctas, FIXUP_STAGES<16>);
+            const Run run = make_run(tiles, steps, b, n, FIXUP_STAGES<16>);
             int seen = 0;
             for (int i = 0; i < run.pieces; ++i) {
                 const Piece q = piece_of(run, i);
@@ -1404,7 +1427,7 @@ int walk_division(int kernel, int tiles, int k_steps, int ctas, int* cover, int*
         for (int t = 0; t < tiles; ++t)
             if (parts[t]) {                              // the count that the last CTA waits to see
                 ++*cut;
-                const Run run = make_run(tiles, k_steps, 0, ctas, FIXUP_STAGES<16>);
+                const Run run = make_run(tiles, steps, 0, n, FIXUP_STAGES<16>);
                 if (parts[t] != owner(run, t * k_steps + k_steps - 1) - owner(run, t * k_steps) + 1) return 105;
             }
         return WUSH_OK;
