@@ -58,7 +58,7 @@ __device__ __forceinline__ uint32_t same_expert(int e, int bits)
     return same;
 }
 
-template <typename Id, int CTAS>
+template <typename Id, int CTAS, bool KEEP>      // KEEP: no warp has more than AHEAD rounds, so ids and ranks stay in registers
 __global__ void __launch_bounds__(SORT_THREADS) expert_sort_kernel(const Id* __restrict__ ids, int64_t n, int E,
                                                                    int32_t* __restrict__ pos, int32_t* __restrict__ offsets)
 {
@@ -82,19 +82,19 @@ __global__ void __launch_bounds__(SORT_THREADS) expert_sort_kernel(const Id* __r
     for (int i = tid; i < warps * E; i += SORT_THREADS) cnt[i] = 0;
     __syncthreads();
     int32_t* mine = cnt + warp * E;
+    int e[AHEAD], at[AHEAD];
     for (int64_t i = first; i < end; i += 32 * AHEAD) {
-        int e[AHEAD];
 #pragma unroll
         for (int a = 0; a < AHEAD; ++a) e[a] = expert_of(ids, i + 32 * a + lane, end, E);
 #pragma unroll
         for (int a = 0; a < AHEAD; ++a) {
             if (i + 32 * a >= end) break;
             const uint32_t same = same_expert(e[a], bits), lower = same & ((1u << lane) - 1);
-            const int32_t at = e[a] >= 0 ? mine[e[a]] + __popc(lower) : -1;          // rank within the run
+            at[a] = e[a] >= 0 ? mine[e[a]] + __popc(lower) : -1;                      // rank within the run
             __syncwarp();
             if (e[a] >= 0 && lower == 0) mine[e[a]] += __popc(same);
             __syncwarp();
-            if (i + 32 * a + lane < end) pos[i + 32 * a + lane] = at;
+            if (!KEEP && i + 32 * a + lane < end) pos[i + 32 * a + lane] = at[a];
         }
     }
     __syncthreads();
@@ -142,15 +142,16 @@ __global__ void __launch_bounds__(SORT_THREADS) expert_sort_kernel(const Id* __r
     }
     __syncthreads();
     for (int64_t i = first + lane; i < end; i += 32 * AHEAD) {                        // every thread its own entries again
-        int e[AHEAD], at[AHEAD];
+        if (!KEEP) {
 #pragma unroll
-        for (int a = 0; a < AHEAD; ++a) {
-            e[a] = expert_of(ids, i + 32 * a, end, E);
-            at[a] = e[a] >= 0 ? pos[i + 32 * a] : 0;
+            for (int a = 0; a < AHEAD; ++a) {
+                e[a] = expert_of(ids, i + 32 * a, end, E);
+                at[a] = e[a] >= 0 ? pos[i + 32 * a] : -1;
+            }
         }
 #pragma unroll
         for (int a = 0; a < AHEAD; ++a)
-            if (e[a] >= 0) pos[i + 32 * a] = mine[e[a]] + at[a];
+            if (i + 32 * a < end) pos[i + 32 * a] = e[a] >= 0 ? mine[e[a]] + at[a] : -1;
     }
     if constexpr (CTAS > 1) cluster_barrier();      // no CTA leaves while its totals may be read
 }
@@ -197,7 +198,7 @@ int launch_sort(const Id* ids, int64_t n, int E, int32_t* pos, int32_t* offsets,
     }
     const size_t smem = sort_smem_bytes(E);
     if (n <= 2048) {                                // 2048 entries: 5.5 us in one CTA, 7 in a cluster; 4096: 7.5 and 7
-        expert_sort_kernel<Id, 1><<<1, SORT_THREADS, smem, st>>>(ids, n, E, pos, offsets);
+        expert_sort_kernel<Id, 1, true><<<1, SORT_THREADS, smem, st>>>(ids, n, E, pos, offsets);
         return check_launch("expert_sort");
     }
     cudaLaunchConfig_t cfg = {};
@@ -212,7 +213,9 @@ int launch_sort(const Id* ids, int64_t n, int E, int32_t* pos, int32_t* offsets,
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    cudaError_t e = cudaLaunchKernelEx(&cfg, expert_sort_kernel<Id, SORT_CLUSTER>, ids, n, E, pos, offsets);
+    const bool keep = n <= (int64_t)32 * AHEAD * SORT_WARPS * SORT_CLUSTER;
+    cudaError_t e = cudaLaunchKernelEx(&cfg, keep ? expert_sort_kernel<Id, SORT_CLUSTER, true> : expert_sort_kernel<Id, SORT_CLUSTER, false>,
+                                       ids, n, E, pos, offsets);
     if (e != cudaSuccess) return fail(WUSH_ERR_CUDA, "expert_sort: launch failed: %s", cudaGetErrorString(e));
     return WUSH_OK;
 }
@@ -260,7 +263,7 @@ __global__ void __launch_bounds__(256) expert_gather_kernel(const Pack<T, N>* __
     const int64_t t = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
     if (t < tokens) {
         constexpr int U = steps_at_once<T, N>();
-        for (int v = threadIdx.x; v < n_vec; v += U * blockDim.x) {
+        for (int v = threadIdx.x + blockIdx.y * U * blockDim.x; v < n_vec; v += U * blockDim.x * gridDim.y) {
             Pack<T, N> p[U];
 #pragma unroll
             for (int u = 0; u < U; ++u) p[u] = x[t * n_vec + min(v + u * (int)blockDim.x, n_vec - 1)];
@@ -273,7 +276,8 @@ __global__ void __launch_bounds__(256) expert_gather_kernel(const Pack<T, N>* __
             }
         }
     }
-    zero_tail(rows, n_vec, *n_used, tokens * k, blockIdx.x, gridDim.x, threadIdx.y * blockDim.x + threadIdx.x, blockDim.x * blockDim.y);
+    zero_tail(rows, n_vec, *n_used, tokens * k, blockIdx.x * gridDim.y + blockIdx.y, gridDim.x * gridDim.y, threadIdx.y * blockDim.x + threadIdx.x,
+              blockDim.x * blockDim.y);
 }
 
 // AT entries of a token at once: their rows are loaded together.  An absent entry loads row 0 and adds nothing: a branch
@@ -332,7 +336,7 @@ __global__ void __launch_bounds__(256, AT <= 4 ? 4 : 3) expert_combine_kernel(co
     pdl_launch_dependents();
     if (t >= tokens) return;
     constexpr int U = steps_at_once<T, N>();
-    for (int v = threadIdx.x; v < n_vec; v += U * blockDim.x) {
+    for (int v = threadIdx.x + blockIdx.y * U * blockDim.x; v < n_vec; v += U * blockDim.x * gridDim.y) {
         float acc[U][N];
 #pragma unroll
         for (int u = 0; u < U; ++u)
@@ -414,8 +418,23 @@ __global__ void __launch_bounds__(256, AT <= 4 || steps_at_once<T, N>() > 1 ? 4 
     zero_tail(d_rows, n_vec, *n_used, tokens * k, blockIdx.x, gridDim.x, tid, blockDim.x);
 }
 
-// Threads along a row of n_vec packs of which a thread takes `at_once`: of 32, 64, 128, 256 the count that leaves the fewest
-// idle in the last step, the largest of equals.
+// Shape of a launch over `tokens` rows of n_vec packs, of which a thread takes `at_once`: blocks of x threads along the row and
+// 256 / x tokens.  The fewest steps weighted by the blocks that have to wait for a place (four per multiprocessor); few
+// tokens get blocks along the row too (221 x 3328 fp32, k = 2: combine 5.8 us with 64 x 4 threads, 2.3 so).
+struct Shape {
+    dim3 grid, block;
+};
+Shape shape_of(int64_t tokens, int64_t n_vec, int at_once)
+{
+    const int64_t n = (n_vec + at_once - 1) / at_once, places = 4 * sm_count();
+    int64_t best = 0, x = 32;
+    for (int t = 32; t <= 256; t *= 2) {
+        const int64_t blocks = (tokens * t + 255) / 256, cost = (n + t - 1) / t * (blocks > places ? blocks : places);
+        if (t == 32 || cost <= best) { best = cost; x = t; }
+    }
+    const int64_t blocks = (tokens * x + 255) / 256, steps = (n + x - 1) / x, y = places / blocks;
+    return {dim3((unsigned)blocks, (unsigned)(y < 1 ? 1 : y < steps ? y : steps)), dim3((unsigned)x, (unsigned)(256 / x))};
+}
 int threads_along(int64_t n_vec, int at_once)
 {
     const int64_t n = (n_vec + at_once - 1) / at_once;
@@ -475,8 +494,9 @@ template <typename T, int N>
 int launch_gather(Pack<T, N>, const void* x, int64_t tokens, int64_t H, const int32_t* pos, int k, const int32_t* n_used, void* rows,
                   cudaStream_t st)
 {
-    const int n_vec = (int)(H / N), tx = threads_along(n_vec, steps_at_once<T, N>()), ty = 256 / tx;
-    expert_gather_kernel<T, N><<<(unsigned)((tokens + ty - 1) / ty), dim3(tx, ty), 0, st>>>((const Pack<T, N>*)x, tokens, n_vec, pos, k,
+    const int n_vec = (int)(H / N);
+    const Shape s = shape_of(tokens, n_vec, steps_at_once<T, N>());
+    expert_gather_kernel<T, N><<<s.grid, s.block, 0, st>>>((const Pack<T, N>*)x, tokens, n_vec, pos, k,
                                                                                         n_used, (Pack<T, N>*)rows);
     return check_launch("expert_gather");
 }
@@ -484,8 +504,9 @@ template <typename T, typename O, int N, int AT>
 int launch_combine_at(const void* rows, int64_t tokens, int64_t H, const int32_t* pos, int k, const float* weights, void* y,
                       bool dependent, cudaStream_t st)
 {
-    const int n_vec = (int)(H / N), tx = threads_along(n_vec, steps_at_once<T, N>()), ty = 256 / tx;
-    const dim3 grid((unsigned)((tokens + ty - 1) / ty)), block(tx, ty);
+    const int n_vec = (int)(H / N);
+    const Shape s = shape_of(tokens, n_vec, steps_at_once<T, N>());
+    const dim3 grid = s.grid, block = s.block;
     if (dependent) {
         cudaError_t e = launch_dependent(expert_combine_kernel<T, O, N, AT>, grid, block, 0, st, (const Pack<T, N>*)rows, tokens, n_vec, pos, k,
                                          weights, (Pack<O, N>*)y);
@@ -533,12 +554,16 @@ int check_moves(const char* op, int dtype, int64_t tokens, int64_t H)
 int expert_order_set_attributes()
 {
     const int most = (int)sort_smem_bytes(WUSH_EXPERT_MAX);
-    cudaError_t e = cudaFuncSetAttribute(expert_sort_kernel<int32_t, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(expert_sort_kernel<int64_t, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
-    if (e == cudaSuccess)
-        e = cudaFuncSetAttribute(expert_sort_kernel<int32_t, SORT_CLUSTER>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
-    if (e == cudaSuccess)
-        e = cudaFuncSetAttribute(expert_sort_kernel<int64_t, SORT_CLUSTER>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+    cudaError_t e = cudaSuccess;
+    auto set = [&](auto kernel) {
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+    };
+    set(expert_sort_kernel<int32_t, 1, true>);
+    set(expert_sort_kernel<int64_t, 1, true>);
+    set(expert_sort_kernel<int32_t, SORT_CLUSTER, true>);
+    set(expert_sort_kernel<int64_t, SORT_CLUSTER, true>);
+    set(expert_sort_kernel<int32_t, SORT_CLUSTER, false>);
+    set(expert_sort_kernel<int64_t, SORT_CLUSTER, false>);
     if (e != cudaSuccess) return fail(WUSH_ERR_CUDA, "expert_sort: cudaFuncSetAttribute failed: %s", cudaGetErrorString(e));
     return WUSH_OK;
 }

@@ -321,6 +321,7 @@ __device__ __forceinline__ void zero_tail(const Params& p, int64_t used, int tid
 // The usual last one is the CTA whose run ends inside the tile: the next CTA began its run with the rest of it.  It looks
 // at the count before its own sums are complete, and where all the others are in it adds their slots to its accumulator
 // and stores nothing (4096 x 24576: 24 tokens 24.9 -> 23.4 us, 64 tokens 29.1 -> 27.2 us).
+template <int NT> constexpr int FIXUP_CTAS = NT == 64 ? 8 : 16;    // at most so many CTAs per cut tile, or one more by uneven borders
 template <int NT> constexpr int FIXUP_STAGES = NT <= 32 ? 12 : 28;      // one token: 2048 x 8192 11.0 us uncut, 11.8 cut; 64 tokens: 4096 x 4096 15.9 and 18.0
 
 struct Run {
@@ -329,17 +330,18 @@ struct Run {
     int k_steps, first;          // stages of a tile; tile of the first stage
     int pieces;                  // tiles and parts of tiles in the run
 };
-__host__ __device__ inline Run make_run(int tiles, const Divisor& steps, int cta, const Divisor& ctas, int fixup)
+__host__ __device__ inline Run make_run(int tiles, const Divisor& steps, int cta, const Divisor& ctas, int fixup, int most)
 {
     Run r;
     const int k_steps = (int)steps.d, n = (int)ctas.d, total = tiles * k_steps, per = divide(tiles, ctas), more = tiles - per * n;
     r.k_steps = k_steps;
-    r.size = divide(total, ctas);
-    r.longer = total - r.size * n;
+    const int used = tiles < n / most ? max(1, tiles * most) : n;
+    r.size = used == n ? divide(total, ctas) : total / used;
+    r.longer = total - r.size * used;
     const int whole = (per + (more ? 1 : 0)) * k_steps, even = r.size + (r.longer ? 1 : 0) + fixup;
     if (whole > even) {          // a CTA without a stage of its own (total < ctas) has an empty run
-        r.begin = cta * r.size + min(cta, r.longer);
-        r.end = r.begin + r.size + (cta < r.longer ? 1 : 0);
+        r.begin = cta < used ? cta * r.size + min(cta, r.longer) : total;
+        r.end = cta < used ? r.begin + r.size + (cta < r.longer ? 1 : 0) : total;
         r.first = divide(r.begin, steps);
         r.pieces = r.end > r.begin ? divide(r.end - 1, steps) - r.first + 1 : 0;
     } else {
@@ -376,25 +378,26 @@ __device__ __forceinline__ int ld_acquire(const int32_t* p)
     asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
     return v;
 }
-// Adds columns [c0, c0 + 16) of channel c from the slots of CTAs c_first..c_last but `own`, four slots at once: one after
-// another they take a trip to L2 each (4096 x 4096, 64 tokens, five CTAs per tile: 21.5 us, 18.0 with this).
+// Adds columns [c0, c0 + 16) of channel c from the slots of CTAs c_first..c_last but `own`, eight slots at once: one after
+// another they take a trip to L2 each (4096 x 4096, 64 tokens, five CTAs per tile: 21.5 us, 18.0 with four at once).
 template <int NT>
 __device__ __forceinline__ void add_slots(const Params& p, uint32_t* v, int c0, int c, int c_first, int c_last, int own)
 {
-    for (int k = c_first; k <= c_last; k += 4) {
+    constexpr int SLOTS = 8;
+    for (int k = c_first; k <= c_last; k += SLOTS) {
 #pragma unroll
         for (int h = 0; h < 16; h += 8) {
-            uint32_t u[4][8];
+            uint32_t u[SLOTS][8];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
+            for (int i = 0; i < SLOTS; ++i) {
                 const int at = min(k + i, c_last);
                 const uint32_t* from = p.pieces + (size_t)(2 * at + (at == c_first)) * Stream<NT>::PIECE + (c0 + h) * 128 + c;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) u[i][j] = __ldcg(from + j * 128);
+                for (int j = 0; j < 8; ++j) u[i][j] = k + i <= c_last ? __ldcg(from + j * 128) : 0u;
             }
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (k + i <= c_last && k + i != own)
+            for (int i = 0; i < SLOTS; ++i)
+                if (k + i != own)
 #pragma unroll
                     for (int j = 0; j < 8; ++j) v[h + j] += u[i][j];
         }
@@ -467,7 +470,7 @@ __global__ void __launch_bounds__(THREADS, 1) w8a8_stream_kernel(const __grid_co
     const uint32_t tmem = *tmem_slot;
     const int k_steps = (int)p.steps.d;
     const int n_tiles = p.offsets ? first_s[p.experts] : ((int)p.rows + NT - 1) / NT * p.tiles_c;
-    const Run run = make_run(n_tiles, p.steps, blockIdx.x, p.ctas, FIXUP_STAGES<NT>);
+    const Run run = make_run(n_tiles, p.steps, blockIdx.x, p.ctas, FIXUP_STAGES<NT>, FIXUP_CTAS<NT>);
     const int e_first = p.offsets ? expert_of_tile(p, first_s, run.first) : 0;
     StreamOrder<NT> order = {p, p.offsets ? first_s : nullptr, row_s, e_first};
     constexpr int WIDTH = GATED ? 64 : 128;
@@ -1409,7 +1412,7 @@ int walk_division(int kernel, int tiles, int k_steps, int ctas, int* cover, int*
         const Divisor steps = make_divisor(k_steps), n = make_divisor(ctas);
         std::vector<int> parts(tiles, 0), slots(2 * (size_t)ctas, 0);
         for (int b = 0; b < ctas; ++b) {
-            const Run run = make_run(tiles, steps, b, n, FIXUP_STAGES<16>);
+            const Run run = make_run(tiles, steps, b, n, FIXUP_STAGES<16>, FIXUP_CTAS<64>);
             int seen = 0;
             for (int i = 0; i < run.pieces; ++i) {
                 const Piece q = piece_of(run, i);
@@ -1427,7 +1430,7 @@ int walk_division(int kernel, int tiles, int k_steps, int ctas, int* cover, int*
         for (int t = 0; t < tiles; ++t)
             if (parts[t]) {                              // the count that the last CTA waits to see
                 ++*cut;
-                const Run run = make_run(tiles, steps, 0, n, FIXUP_STAGES<16>);
+                const Run run = make_run(tiles, steps, 0, n, FIXUP_STAGES<16>, FIXUP_CTAS<64>);
                 if (parts[t] != owner(run, t * k_steps + k_steps - 1) - owner(run, t * k_steps) + 1) return 105;
             }
         return WUSH_OK;
