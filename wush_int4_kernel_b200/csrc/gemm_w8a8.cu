@@ -321,7 +321,8 @@ __device__ __forceinline__ void zero_tail(const Params& p, int64_t used, int tid
 // The usual last one is the CTA whose run ends inside the tile: the next CTA began its run with the rest of it.  It looks
 // at the count before its own sums are complete, and where all the others are in it adds their slots to its accumulator
 // and stores nothing (4096 x 24576: 24 tokens 24.9 -> 23.4 us, 64 tokens 29.1 -> 27.2 us).
-template <int NT> constexpr int FIXUP_CTAS = NT == 64 ? 8 : 16;    // at most so many CTAs per cut tile, or one more by uneven borders
+// At most so many CTAs per cut tile (one more where borders are uneven): 16 x 4096 -> 1024 takes 8.7 us with 8, 9.4 with 16.
+constexpr int FIXUP_CTAS = 8;
 template <int NT> constexpr int FIXUP_STAGES = NT <= 32 ? 12 : 28;      // one token: 2048 x 8192 11.0 us uncut, 11.8 cut; 64 tokens: 4096 x 4096 15.9 and 18.0
 
 struct Run {
@@ -378,29 +379,37 @@ __device__ __forceinline__ int ld_acquire(const int32_t* p)
     asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
     return v;
 }
-// Adds columns [c0, c0 + 16) of channel c from the slots of CTAs c_first..c_last but `own`, eight slots at once: one after
-// another they take a trip to L2 each (4096 x 4096, 64 tokens, five CTAs per tile: 21.5 us, 18.0 with four at once).
+// Slots hold four token columns of a channel side by side, so that a lane moves 16 bytes: with single words the last CTA of a
+// tile spent 8 us on nine pieces of 32 tokens (24 x 8192 -> 2048: 17.2 us, 13.7 with these).
+__device__ __forceinline__ void put_columns(uint32_t* slot, int col, int c, const uint32_t* v)
+{
+    __stcg(reinterpret_cast<uint4*>(slot) + (col / 4) * 128 + c, make_uint4(v[0], v[1], v[2], v[3]));
+}
+__device__ __forceinline__ uint4 get_columns(const uint32_t* slot, int col, int c)
+{
+    return __ldcg(reinterpret_cast<const uint4*>(slot) + (col / 4) * 128 + c);
+}
+__device__ __forceinline__ void add4(uint32_t* v, const uint4& u) { v[0] += u.x; v[1] += u.y; v[2] += u.z; v[3] += u.w; }
+
+// Adds columns [c0, c0 + 16) of channel c from the slots of CTAs c_first..c_last but `own`, four slots at once.
 template <int NT>
 __device__ __forceinline__ void add_slots(const Params& p, uint32_t* v, int c0, int c, int c_first, int c_last, int own)
 {
-    constexpr int SLOTS = 8;
+    constexpr int SLOTS = 4;
     for (int k = c_first; k <= c_last; k += SLOTS) {
+        uint4 u[SLOTS][4];
 #pragma unroll
-        for (int h = 0; h < 16; h += 8) {
-            uint32_t u[SLOTS][8];
+        for (int i = 0; i < SLOTS; ++i) {
+            const int at = min(k + i, c_last);
+            const uint32_t* slot = p.pieces + (size_t)(2 * at + (at == c_first)) * Stream<NT>::PIECE;
 #pragma unroll
-            for (int i = 0; i < SLOTS; ++i) {
-                const int at = min(k + i, c_last);
-                const uint32_t* from = p.pieces + (size_t)(2 * at + (at == c_first)) * Stream<NT>::PIECE + (c0 + h) * 128 + c;
-#pragma unroll
-                for (int j = 0; j < 8; ++j) u[i][j] = k + i <= c_last ? __ldcg(from + j * 128) : 0u;
-            }
-#pragma unroll
-            for (int i = 0; i < SLOTS; ++i)
-                if (k + i != own)
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) v[h + j] += u[i][j];
+            for (int j = 0; j < 4; ++j) u[i][j] = get_columns(slot, c0 + 4 * j, c);
         }
+#pragma unroll
+        for (int i = 0; i < SLOTS; ++i)
+            if (k + i <= c_last && k + i != own)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) add4(v + 4 * j, u[i][j]);
     }
 }
 
@@ -470,7 +479,7 @@ __global__ void __launch_bounds__(THREADS, 1) w8a8_stream_kernel(const __grid_co
     const uint32_t tmem = *tmem_slot;
     const int k_steps = (int)p.steps.d;
     const int n_tiles = p.offsets ? first_s[p.experts] : ((int)p.rows + NT - 1) / NT * p.tiles_c;
-    const Run run = make_run(n_tiles, p.steps, blockIdx.x, p.ctas, FIXUP_STAGES<NT>, FIXUP_CTAS<NT>);
+    const Run run = make_run(n_tiles, p.steps, blockIdx.x, p.ctas, FIXUP_STAGES<NT>, FIXUP_CTAS);
     const int e_first = p.offsets ? expert_of_tile(p, first_s, run.first) : 0;
     StreamOrder<NT> order = {p, p.offsets ? first_s : nullptr, row_s, e_first};
     constexpr int WIDTH = GATED ? 64 : 128;
@@ -576,7 +585,7 @@ __global__ void __launch_bounds__(THREADS, 1) w8a8_stream_kernel(const __grid_co
             if (ok) ok = __all_sync(0xffffffffu, tc::mbar_wait(&acc_full[ab], aphase));
             tc::tc_fence_after();
             const uint32_t base = tmem + ((uint32_t)(quarter * 32) << 16) + ab * NT;
-            uint32_t* slot = p.pieces + (size_t)(2 * blockIdx.x + (q.k0 == 0)) * C::PIECE + c;
+            uint32_t* slot = p.pieces + (size_t)(2 * blockIdx.x + (q.k0 == 0)) * C::PIECE;
 #pragma unroll
             for (int c0 = 0; c0 < NT; c0 += 16) {
                 uint32_t v[16];
@@ -592,7 +601,7 @@ __global__ void __launch_bounds__(THREADS, 1) w8a8_stream_kernel(const __grid_co
                     if (ok) emit<GATED, 16>(p, L, c0, v);
                 } else {
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) __stcg(slot + (c0 + j) * 128, v[j]);
+                    for (int j = 0; j < 16; j += 4) put_columns(slot, c0 + j, c, v + j);
                 }
             }
             if (!whole && !last) {
@@ -926,9 +935,9 @@ w8a8_pair_kernel(const __grid_constant__ PairMaps maps, const Params p, int band
                 if (whole) {
                     emit<GATED, 32>(p, now, c0 * 32, v);
                 } else {
-                    uint32_t* slot = p.pieces + ((size_t)blockIdx.x * PAIR_TOKENS + c0 * 32) * 128 + c;
+                    uint32_t* slot = p.pieces + (size_t)blockIdx.x * PAIR_TOKENS * 128;
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) __stcg(slot + j * 128, v[j]);
+                    for (int j = 0; j < 32; j += 4) put_columns(slot, c0 * 32 + j, c, v + j);
                 }
             }
             if (half >= chunks && lane == 0) mbar_arrive_cluster_relaxed(tc::map_to_rank(&acc_empty[ab], 0));
@@ -972,21 +981,22 @@ __global__ void __launch_bounds__(128) w8a8_tail_kernel(const Params p, int band
     Lane L = make_lane<GATED>(p, tile, (int64_t)tile.ct * 2 * WIDTH + rank * WIDTH, c, sx_s - c0);
     if (c < TAIL_TOKENS) sx_s[c] = c0 + c < tile.n_rows ? p.xs[tile.row0 + c0 + c] : 0.f;
     __syncthreads();
-    const uint32_t* from = p.pieces + ((size_t)(2 * t * tail.split + rank) * PAIR_TOKENS + c0) * 128 + c;
+    const uint32_t* slots = p.pieces + (size_t)(2 * t * tail.split + rank) * PAIR_TOKENS * 128;
     uint32_t v[TAIL_TOKENS];
 #pragma unroll
     for (int j = 0; j < TAIL_TOKENS; ++j) v[j] = 0;
     for (int s = 0; s < tail.split; s += 4) {
-        uint32_t u[4][TAIL_TOKENS];
+        uint4 u[4][TAIL_TOKENS / 4];
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
-            for (int j = 0; j < TAIL_TOKENS; ++j) u[i][j] = __ldcg(from + (size_t)min(s + i, tail.split - 1) * (2 * PAIR_TOKENS * 128) + j * 128);
+            for (int j = 0; j < TAIL_TOKENS / 4; ++j)
+                u[i][j] = get_columns(slots + (size_t)min(s + i, tail.split - 1) * (2 * PAIR_TOKENS * 128), c0 + 4 * j, c);
 #pragma unroll
         for (int i = 0; i < 4; ++i)
             if (s + i < tail.split)
 #pragma unroll
-                for (int j = 0; j < TAIL_TOKENS; ++j) v[j] += u[i][j];
+                for (int j = 0; j < TAIL_TOKENS / 4; ++j) add4(v + 4 * j, u[i][j]);
     }
     emit<GATED, TAIL_TOKENS>(p, L, c0, v);
 }
@@ -1412,7 +1422,7 @@ int walk_division(int kernel, int tiles, int k_steps, int ctas, int* cover, int*
         const Divisor steps = make_divisor(k_steps), n = make_divisor(ctas);
         std::vector<int> parts(tiles, 0), slots(2 * (size_t)ctas, 0);
         for (int b = 0; b < ctas; ++b) {
-            const Run run = make_run(tiles, steps, b, n, FIXUP_STAGES<16>, FIXUP_CTAS<64>);
+            const Run run = make_run(tiles, steps, b, n, FIXUP_STAGES<16>, FIXUP_CTAS);
             int seen = 0;
             for (int i = 0; i < run.pieces; ++i) {
                 const Piece q = piece_of(run, i);
@@ -1430,7 +1440,7 @@ int walk_division(int kernel, int tiles, int k_steps, int ctas, int* cover, int*
         for (int t = 0; t < tiles; ++t)
             if (parts[t]) {                              // the count that the last CTA waits to see
                 ++*cut;
-                const Run run = make_run(tiles, steps, 0, n, FIXUP_STAGES<16>, FIXUP_CTAS<64>);
+                const Run run = make_run(tiles, steps, 0, n, FIXUP_STAGES<16>, FIXUP_CTAS);
                 if (parts[t] != owner(run, t * k_steps + k_steps - 1) - owner(run, t * k_steps) + 1) return 105;
             }
         return WUSH_OK;
