@@ -1,7 +1,7 @@
 """Measurement matrix over the layer shapes the reference quotes (``bench/exp_p13_official.py:42-63``
 draws random tensors of the same shapes; no dataset or checkpoint is involved).
 
-    python -m wush_int4_kernel_b200.bench_matrix [--configs qwen,llama,mid,square,prefill,ffn] [--tp P]
+    python -m wush_int4_kernel_b200.bench_matrix [--configs qwen,llama,mid,square,prefill,ffn,int8,experts] [--tp P]
     torchrun --nproc-per-node P -m wush_int4_kernel_b200.bench_matrix --configs ffn
 
 For every (K, N, M) one JSON line with the time of the fused transform+quantisation, of the
@@ -14,6 +14,10 @@ batches of 100 (M <= 4), 30 (M <= 256) or 8 replays.
 ``ffn`` times the Llama-70B FFN block (hidden 8192, intermediate 28672) of ONE tensor-parallel
 rank: under torchrun with P ranks including the all-reduce of the down projection, otherwise
 (``--tp P``) the compute of rank 0's shard alone.
+
+``int8`` times the 8-bit layer (quantiser and product in one call) on the decode and prefill sizes of the
+70B gate+up projection, ``experts`` the 8-bit mixture-of-experts block; the peak of a row is the larger of
+the bytes of the weights it reaches at the HBM copy bandwidth and its operations at dense int8 throughput.
 """
 from __future__ import annotations
 
@@ -202,6 +206,53 @@ def measure_column_gather(M: int, tp: int, rank: int, dev, peer, layers) -> dict
                       ("peer memory, pushed from the product kernel" if M <= 32 else "peer memory, one kernel")}
 
 
+INT8_SHAPES = ((8192, 57344, (1, 16, 64, 128, 512, 4096)), (28672, 8192, (1, 333)))                # (K, N, rows per step)
+EXPERT_SHAPES = ((2048, 1024, 64, 8, (1, 16, 128, 4096)), (4096, 7168, 8, 2, (1, 32, 777)))        # (H, I, experts, k, tokens)
+
+
+def _int8_weights(*shape, gen):
+    q = torch.randint(-127, 128, shape, generator=gen, device="cuda", dtype=torch.int8)
+    return q, 1e-3 * (0.5 + torch.rand(shape[:-1], generator=gen, device="cuda"))
+
+
+def _int8_line(what: dict, steps: list, M: int, weight_bytes: float, ops: float) -> dict:
+    from . import timing
+
+    us = _median_us([timing.capture(step)[0] for step in steps], _reps(M))
+    bound = max(weight_bytes / _hbm_peak()[0] / 1e3, ops / INT8_NOMINAL_TOPS / 1e6)
+    return what | {"us": round(us, 2), "tops": round(ops / us / 1e6, 1), "bound_us": round(bound, 2), "of_bound": round(bound / us, 3)}
+
+
+def measure_int8(emit) -> None:
+    """One line per shape of the 8-bit layer, weights rotated as for the 4-bit one."""
+    from .linear import W8A8Linear
+
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    for K, N, rows in INT8_SHAPES:
+        layers = [W8A8Linear(*_int8_weights(N, K, gen=gen)) for _ in range(max(2, 2 + (2 * L2_BYTES) // (N * K)))]
+        for M in rows:
+            x = torch.randn(M, K, generator=gen, device="cuda").to(torch.bfloat16)
+            emit(_int8_line({"layer": "w8a8", "K": K, "N": N, "M": M}, [lambda l=l: l(x) for l in layers], M, float(N * K), 2.0 * M * N * K))
+        del layers
+
+
+def measure_experts(emit) -> None:
+    """One line per shape of the 8-bit mixture-of-experts block under a router without favourites."""
+    from .experts import W8A8Experts
+
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    for H, inner, E, k, tokens in EXPERT_SHAPES:
+        blocks = [W8A8Experts(*_int8_weights(E, 2 * inner, H, gen=gen), *_int8_weights(E, H, inner, gen=gen)) for _ in range(2)]
+        for T in tokens:
+            x = torch.randn(T, H, generator=gen, device="cuda").to(torch.bfloat16)
+            top, ids = torch.randn(T, E, generator=gen, device="cuda").topk(k, dim=-1)
+            w = torch.softmax(top, dim=-1)
+            reached = int(ids.unique().numel())
+            emit(_int8_line({"layer": "w8a8_experts", "H": H, "I": inner, "E": E, "k": k, "T": T}, [lambda b=b: b(x, ids, w) for b in blocks],
+                            T, 3.0 * reached * H * inner, 6.0 * T * k * H * inner))
+        del blocks
+
+
 def main():
     ap = argparse.ArgumentParser()
     ap.add_argument("--configs", default="qwen,llama,square,prefill")
@@ -229,6 +280,9 @@ def main():
                 line = measure_ffn(m, world if world > 1 else args.tp, rank if world > 1 else 0, dev, world > 1, peer)
                 if rank == 0:
                     print(json.dumps(line), flush=True)
+        elif name in ("int8", "experts"):
+            if world == 1:
+                (measure_int8 if name == "int8" else measure_experts)(lambda line: print(json.dumps(line), flush=True))
         elif world == 1:
             K, N, rows = SHAPES[name]
             layers = make_copies(K, N, dev)

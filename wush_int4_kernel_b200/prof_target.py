@@ -7,6 +7,9 @@ small, self-contained process to capture.
     python -m wush_int4_kernel_b200.prof_target gemm_v VARIANT M N K [reps]   (C ABI, variant gemv|decode|decode_tc|tile|tile_f16)
     python -m wush_int4_kernel_b200.prof_target fused M K   [reps]
     python -m wush_int4_kernel_b200.prof_target quant M K   [reps]
+    python -m wush_int4_kernel_b200.prof_target w8a8  M N K [reps]           (8-bit layer: quantiser and product)
+    python -m wush_int4_kernel_b200.prof_target experts T H I E k [reps]     (8-bit mixture-of-experts block)
+    python -m wush_int4_kernel_b200.prof_target expert_grad T H E k [reps]   (gradients of the weighted sum and of the gather)
 
 Prints the mean time per call measured with CUDA events (never quote a time taken under a
 profiler).
@@ -24,6 +27,11 @@ def _codes(rows, K, gen, dev):
     q = torch.randint(0, 256, (rows, K // 2), generator=gen, device=dev, dtype=torch.uint8)
     s = (0.01 * (1 + 0.5 * torch.rand(rows, K // 32, generator=gen, device=dev))).to(torch.bfloat16)
     return q, s
+
+
+def _int8(gen, dev, *shape):
+    q = torch.randint(-127, 128, shape, generator=gen, device=dev, dtype=torch.int8)
+    return q, 1e-3 * (0.5 + torch.rand(shape[:-1], generator=gen, device=dev))
 
 
 def main(argv):
@@ -74,6 +82,36 @@ def main(argv):
         x = torch.randn(M, K, generator=gen, device=dev).to(torch.bfloat16)
         t = (torch.randn(K // 32, 32, 32, generator=gen, device=dev) / 6).to(torch.bfloat16)
         fn = (lambda: _C.fused_transform_quant_int4_v3(x, t)) if op == "fused" else (lambda: _C.quant_int4(x))
+        work = 0.0
+    elif op == "w8a8":
+        from .linear import W8A8Linear
+        M, N, K = map(int, argv[1:4])
+        reps = int(argv[4]) if len(argv) > 4 else 5
+        layer = W8A8Linear(*_int8(gen, dev, N, K))
+        x = torch.randn(M, K, generator=gen, device=dev).to(torch.bfloat16)
+        fn = lambda: layer(x)
+        work = 2.0 * M * N * K
+    elif op == "experts":
+        from .experts import W8A8Experts
+        T, H, inner, E, k = map(int, argv[1:6])
+        reps = int(argv[6]) if len(argv) > 6 else 5
+        block = W8A8Experts(*_int8(gen, dev, E, 2 * inner, H), *_int8(gen, dev, E, H, inner))
+        x = torch.randn(T, H, generator=gen, device=dev).to(torch.bfloat16)
+        top, ids = torch.randn(T, E, generator=gen, device=dev).topk(k, dim=-1)
+        w = torch.softmax(top, dim=-1)
+        fn = lambda: block(x, ids, w)
+        work = 6.0 * T * k * H * inner
+    elif op == "expert_grad":
+        from .experts import ExpertRoute
+        T, H, E, k = map(int, argv[1:5])
+        reps = int(argv[5]) if len(argv) > 5 else 5
+        top, ids = torch.randn(T, E, generator=gen, device=dev).topk(k, dim=-1)
+        route, w = ExpertRoute.sort(ids, E), torch.softmax(top, dim=-1)
+        dy, rows = (torch.randn(n, H, generator=gen, device=dev).to(torch.bfloat16) for n in (T, T * k))
+
+        def fn():
+            d_rows, _ = _C.expert_combine_grad(dy, rows, route.pos, route.offsets, w)
+            _C.expert_combine(d_rows, route.pos)
         work = 0.0
     else:
         raise SystemExit(__doc__)
