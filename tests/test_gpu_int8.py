@@ -511,6 +511,26 @@ def test_grouped_offsets_outside_the_rows_are_cut(C):
     assert torch.equal(y[0], x[0]) and not y[1].any()
 
 
+def test_grouped_most_experts(C):
+    """1024 experts, most of them without a row, through every operator that takes offsets."""
+    from wush_int4_kernel_b200.experts import W8A8Experts
+    g = gen(77)
+    E, H, inner = 1024, 64, 32
+    block = W8A8Experts.from_weights(randn(E, 2 * inner, H, g=g) * H ** -0.5, randn(E, H, inner, g=g) * inner ** -0.5)
+    for T, k in ((3, 2), (40, 64), (700, 64)):
+        ids = torch.randint(0, E, (T, k), generator=g, device="cuda") // 3 * 3
+        x, w = randn(T, H, g=g, dtype=torch.bfloat16), torch.softmax(randn(T, k, g=g), -1)
+        assert torch.equal(block(x, ids, w), block.by_operators(x, ids, w))
+        pos, offsets = C.expert_sort(ids, E)
+        want = order64(ids, E)
+        assert torch.equal(pos, want[0]) and torch.equal(offsets, want[1])
+        xq, xs = C.expert_gather_quant_int8(x, pos, offsets)
+        y = C.w8a8_grouped_gemm(xq, xs, block.w13q, block.w13s, offsets, torch.float32)
+        owner = ids.view(-1)[pos.view(-1).argsort()]                     # expert of each row
+        want = torch.einsum("rk,rnk->rn", xq.double(), block.w13q[owner].double()) * xs.double()[:, None] * block.w13s[owner].double()
+        within(y, want, want.abs() * 4 * U)
+
+
 def test_grouped_refuse(C):
     xq, xs, wq, ws, offsets = grouped_case([3, 4], 0, 32, 64, gen(8))
     for args in ((xq, xs, wq, ws, offsets[:-1]), (xq, xs, wq[0], ws, offsets), (xq, xs, wq, ws[:, :-1], offsets),

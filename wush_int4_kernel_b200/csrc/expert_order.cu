@@ -324,10 +324,11 @@ struct Entries {
 };
 
 template <typename T, typename O, int N, int AT>
-__global__ void __launch_bounds__(256, AT <= 4 ? 4 : 3) expert_combine_kernel(const Pack<T, N>* __restrict__ rows, int64_t tokens, int n_vec,
-                                                             const int32_t* __restrict__ pos, int k,
-                                                             const float* __restrict__ weights, Pack<O, N>* __restrict__ y)
+__global__ void __launch_bounds__(256, AT <= 4 ? 4 : 3) expert_combine_kernel(const Pack<T, N>* rows, int64_t tokens, int n_vec, const int32_t* pos,
+                                                                           int k, const float* weights, Pack<O, N>* y)
 {
+    // No __restrict__: as a dependent launch this kernel runs while the one in front still writes the rows, which rules out the
+    // read-only loads that it would allow.
     const int64_t t = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
     Entries<T, N, AT> first;
     // Positions and weights are not written by the kernel in front: the expert block launches this one beside its last product.

@@ -1,13 +1,13 @@
 // W8A8 product with one scale per token and one per channel, plain, gated and grouped by expert, on tcgen05 kind::i8.
 //
-//   y[m][n] = sx[m] * sw[n] * sum_k qx[m][k] * qw[n][k] (+ bias[n])          plain, fp16 / bf16
+//   y[m][n] = sx[m] * sw[n] * sum_k qx[m][k] * qw[n][k] (+ bias[n])          plain, fp16 / bf16 / fp32
 //   h[m][i] = silu(g) * u, g / u = the products of channels i and I + i       gated, fp32
 //
 // The int32 sums are exact (K <= 131072), so no order of the work shows in a result; the scales are applied once, in fp32.
 //
 // The WEIGHTS are the 128-row operand and the tokens the other one.  A tile then needs no more tokens than there are (16,
 // 32, 64, ... columns of tensor memory instead of 128 rows), which is what decode batches and the ragged row counts of
-// experts want, and one kernel serves all of them.  Bytes of a weight are read once and go from HBM through TMA (128-byte
+// experts want.  Bytes of a weight are read once and go from HBM through TMA (128-byte
 // swizzle) to the tensor core without passing a register; nothing is unpacked.
 //
 // The weight tensor is described to TMA as (K, 2 or 1, channels, experts): a gated tile takes 64 gate rows and the 64 up
@@ -17,7 +17,8 @@
 // Up to 64 tokens per expert: persistent CTAs, one per multiprocessor, that stream weights without a pause (below).
 // More: CTA pairs on 256 x 256 tiles (further down).
 //
-// Roles per CTA (192 threads): warp 0 TMA producer, warp 1 MMA issuer (and owner of the tensor memory), warps 2-5 epilogue.
+// Roles per CTA: warp 0 TMA producer, warp 1 MMA issuer (and owner of the tensor memory), the others epilogue (four warps in
+// the streaming kernel, eight in the pair kernel).
 // Every wait is bounded; one that gives up leaves a role code in a device word (wush_device_flag, bits 16-23).
 #include <algorithm>
 #include <new>
@@ -608,6 +609,7 @@ __global__ void __launch_bounds__(THREADS, 1) w8a8_stream_kernel(const __grid_co
                 __threadfence();
                 asm volatile("bar.sync 1, 128;" ::: "memory");
                 if (tid == 64) {
+                    __threadfence();
                     last_s[ab] = atomicAdd(p.counters + c_first, 1) == c_last - c_first;
                     __threadfence();
                 }
@@ -1048,7 +1050,7 @@ int launch_stream(const W8A8Problem& w, Params p, bool dependent, cudaStream_t s
     const int64_t most = stream_tiles(w, NT);
     if (most * ((w.K + 127) / 128) > 0x7fffffffll) return fail(WUSH_ERR_UNSUPPORTED, "w8a8: too many tiles (%lld)", (long long)most);
     p.steps = make_divisor((uint32_t)((w.K + 127) / 128));
-    p.ctas = make_divisor((uint32_t)sm_count());
+    p.ctas = make_divisor((uint32_t)std::min<int>(sm_count(), W8A8_COUNTER_BYTES / sizeof(int32_t)));      // a counter per CTA
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(p.ctas.d);
     cfg.blockDim = dim3(THREADS);
@@ -1311,7 +1313,8 @@ WUSH_API int wush_w8a8_linear(const void* x, int dtype, const int8_t* wq, const 
 {
     using namespace wush;
     WUSH_REQUIRE(dtype == WUSH_F16 || dtype == WUSH_BF16, "w8a8_linear: activations are fp16 or bf16");
-    const LinearPlan f = linear_plan(M > 0 ? M : 0, K > 0 ? K : 0);
+    WUSH_REQUIRE(M >= 0 && M < (1ll << 31) && K > 0 && K <= WUSH_W8A8_MAX_K, "w8a8_linear: bad number of rows or K beyond %d", WUSH_W8A8_MAX_K);
+    const LinearPlan f = linear_plan(M, K);
     int8_t* xq = (int8_t*)workspace + f.xq;
     float* xs = (float*)((uint8_t*)workspace + f.xs);
     const W8A8Problem p = {xq, xs, wq, ws, bias, nullptr, M, N, K, 1, false, dtype, y};

@@ -197,11 +197,11 @@ __device__ __forceinline__ void zero_counters(int32_t* counters)
 }
 
 template <typename T>
-__global__ void __launch_bounds__(1024) quant_int8_kernel(const T* __restrict__ x, int64_t rows, int K, int tpr,
-                                                          int8_t* __restrict__ q, float* __restrict__ s,
-                                                          const int32_t* __restrict__ pos, int k,
-                                                          const int32_t* __restrict__ n_used, int32_t* __restrict__ counters)
+__global__ void __launch_bounds__(1024) quant_int8_kernel(const T* x, int64_t rows, int K, int tpr, int8_t* q, float* s, const int32_t* pos,
+                                                          int k, const int32_t* n_used, int32_t* counters)
 {
+    // No __restrict__: as a dependent launch this kernel runs while the one in front still writes x or pos, which rules out
+    // the read-only loads that it would allow.
     __shared__ uint32_t part[32];
     // In front of a gather runs the sort, which writes positions but not the rows to be quantised: those are read at once.
     // Behind a gated product, the product that follows may start at once: before its own wait it reads weights and offsets,
