@@ -598,6 +598,22 @@ def test_same_expert_twice_and_no_token(C):
     assert torch.equal(block(wide, ids, w), block(wide.contiguous(), ids, w))
 
 
+def test_blocks_one_after_another(C):
+    """Calls that follow each other without a pause on the same workspace addresses, each on data of its own."""
+    from wush_int4_kernel_b200.experts import W8A8Experts
+    g = gen(41)
+    E, H, inner = 16, 1024, 528
+    block = W8A8Experts.from_weights(randn(E, 2 * inner, H, g=g, dtype=torch.bfloat16) * H ** -0.5,
+                                     randn(E, H, inner, g=g, dtype=torch.bfloat16) * inner ** -0.5)
+    for T, k in ((2, 4), (60, 4), (300, 2), (900, 5)):
+        sets = [(randn(T, H, g=g, dtype=torch.bfloat16), ids_of(T, k, E, g), torch.softmax(randn(T, k, g=g), -1)) for _ in range(12)]
+        want = [block.by_operators(*s) for s in sets]
+        torch.cuda.synchronize()
+        got = [block(*s) for _ in range(3) for s in sets]
+        for i, y in enumerate(got):
+            assert torch.equal(y, want[i % len(sets)]), (T, k, i)
+
+
 def test_a_large_block_in_a_graph(C):
     """The other kernels of the chain (sort in a cluster, CTA pairs, tiles cut along K) captured, replayed on new inputs."""
     from wush_int4_kernel_b200.experts import W8A8Experts

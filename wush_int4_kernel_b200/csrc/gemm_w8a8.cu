@@ -784,9 +784,8 @@ w8a8_pair_kernel(const __grid_constant__ PairMaps maps, const Params p, int band
     const uint32_t rank = tc::cluster_ctarank();
     const int pair = blockIdx.x >> 1, n_pairs = gridDim.x >> 1;
 
-    pdl_wait();
-    pdl_launch_dependents();
     if (tid == 0) {
+        tc::prefetch_tensormap(&maps.w);
         for (int i = 0; i < PAIR_STAGES; ++i) { tc::mbar_init(&full[i], 1); tc::mbar_init(&empty[i], 1); }
         for (int i = 0; i < PAIR_ACC; ++i) { tc::mbar_init(&acc_full[i], 1); tc::mbar_init(&acc_empty[i], 2 * PAIR_EPILOGUE / 32); }
         tc::mbar_init(done_bar, 1);
@@ -796,6 +795,7 @@ w8a8_pair_kernel(const __grid_constant__ PairMaps maps, const Params p, int band
         tc::tmem_alloc_pair(tmem_slot, 512);
         tc::tmem_relinquish_pair();
     }
+    if (!p.early) pdl_wait();
     if (warp == 0 && p.offsets) make_table(p, first_s, row_s, [](int n) { return token_tiles(n); });
     tc::tc_fence_before();
     __syncthreads();
@@ -823,18 +823,33 @@ w8a8_pair_kernel(const __grid_constant__ PairMaps maps, const Params p, int band
                 const int m = (half + 31) / 32 - 1, row = (int)tile.row0 + (int)rank * half;
                 const uint32_t bytes = 2 * (A_BYTES + (m + 1) * 32 * 128);          // of both CTAs
                 const CUtensorMap* mx = &maps.x[m];
-                for (int ks = w.k0; ks < w.k1; ++ks) {
-                    if (!tc::mbar_wait(&empty[slot], phase ^ 1)) { ok = false; break; }
+                auto load = [&](int ks, bool weights, bool tokens) {                     // of stage ks into the present slot
                     uint8_t* st = smem + slot * PAIR_STAGE;
                     const uint32_t bar = tc::map_to_rank(&full[slot], 0);
                     const int blocks = min(PAIR_BLOCKS, k_blocks - ks * PAIR_BLOCKS);
-                    if (rank == 0) tc::mbar_expect_tx(&full[slot], blocks * bytes);
+                    if (weights && rank == 0) tc::mbar_expect_tx(&full[slot], blocks * bytes);
                     for (int b = 0; b < blocks; ++b) {
                         const int k = (ks * PAIR_BLOCKS + b) * 128;
-                        if (p.weights_once) tma_load_4d_pair(st + b * PAIR_BLOCK, &maps.w, bar, k, 0, c0, tile.expert, policy);
-                        else tma_load_4d_pair(st + b * PAIR_BLOCK, &maps.w, bar, k, 0, c0, tile.expert);
-                        tc::tma_load_2d_pair(st + b * PAIR_BLOCK + A_BYTES, mx, bar, (ks * PAIR_BLOCKS + b) * 128, row);
+                        if (weights) {
+                            if (p.weights_once) tma_load_4d_pair(st + b * PAIR_BLOCK, &maps.w, bar, k, 0, c0, tile.expert, policy);
+                            else tma_load_4d_pair(st + b * PAIR_BLOCK, &maps.w, bar, k, 0, c0, tile.expert);
+                        }
+                        if (tokens) tc::tma_load_2d_pair(st + b * PAIR_BLOCK + A_BYTES, mx, bar, k, row);
                     }
+                };
+                int ks = w.k0;
+                if (i == 0 && p.early) {                                                 // weights do not depend on the kernel in front
+                    const int ahead = min(PAIR_STAGES, w.k1 - w.k0);
+                    for (; slot < (uint32_t)ahead; ++slot) load(ks + slot, true, false);
+                    pdl_wait();
+                    for (slot = 0; slot < (uint32_t)ahead; ++slot) load(ks + slot, false, true);
+                    ks += ahead;
+                    issued = ahead;
+                    if (slot == PAIR_STAGES) { slot = 0; phase = 1; }
+                }
+                for (; ks < w.k1; ++ks) {
+                    if (!tc::mbar_wait(&empty[slot], phase ^ 1)) { ok = false; break; }
+                    load(ks, true, true);
                     ++issued;
                     if (++slot == PAIR_STAGES) { slot = 0; phase ^= 1; }
                 }
@@ -896,6 +911,8 @@ w8a8_pair_kernel(const __grid_constant__ PairMaps maps, const Params p, int band
                 if (tc::mbar_try_wait(done_bar, 0)) break;
         }
     } else {
+        if (p.early) pdl_wait();
+        pdl_launch_dependents();
         const int quarter = warp & 3, c = quarter * 32 + lane;                   // tcgen05.ld: a warp reads lanes 32 * (warp % 4) ...
         const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
         if (p.offsets) zero_tail<GATED>(p, row_s[p.experts], tid - 64, PAIR_EPILOGUE);
